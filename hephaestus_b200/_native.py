@@ -18,6 +18,8 @@ F32, F64, U32, I32, I64 = range(5)
 SUM, PROD, MIN, MAX, MEAN = range(5)
 FORWARD, REVERSE = 0, 1
 MAP_DOT, MAP_SUM, MAP_NORM_L1, MAP_NORM_L2, MAP_NORM_MAX = range(5)
+ROW_F32, ROW_BF16, ROW_F16 = range(3)
+ROUTE_SOFTMAX, ROUTE_SIGMOID = range(2)
 MAX_RANK = 4
 COMM_ID_BYTES = 128
 
@@ -43,6 +45,10 @@ _vp = ctypes.c_void_p
 _u64 = ctypes.c_uint64
 _u32 = ctypes.c_uint32
 _i = ctypes.c_int
+_i32 = ctypes.c_int32
+_i64 = ctypes.c_int64
+_f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _lp = ctypes.POINTER(Layout_t)
 _pp = ctypes.POINTER(ctypes.c_void_p)
 _st = ctypes.c_int  # heph_status
@@ -115,6 +121,16 @@ SIGNATURES = [
     ("heph_scan_host", _st, [_vp, _i, _i, _i, _vp, _vp, _u64, _u64]),
     ("heph_scan_reduce_host", _st, [_vp, _i, _i, _i, _vp, _vp, _u64, _i, _i, _vp, _u64]),
     ("heph_reduce_full_noalloc", _st, [_i, _i, _i, _vp, _u64, _vp, _vp]),
+    ("heph_rms_norm", _st, [_i, _i, _vp, _i64, _vp, _i64, _vp, _i, _f64, _u64, _u64, _vp, _vp, _vp]),
+    ("heph_rms_norm_fp8", _st, [_i, _i, _vp, _i64, _vp, _i64, _vp, _i, _f64, _u64, _u64, _u32, _vp, _vp, _vp, _vp]),
+    ("heph_rms_norm_backward_workspace", _st, [_i, _u64, _u64, ctypes.POINTER(_u64)]),
+    ("heph_rms_norm_backward", _st, [_i, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i, _f64, _u64, _u64, _vp, _vp, _vp,
+                                     _u64, _vp]),
+    ("heph_route_experts", _st, [_i, _i, _vp, _i64, _vp, _u64, _u32, _u32, _i, _u32, _u32, _u32, _i, _f32, _vp, _vp, _vp]),
+    ("heph_route_experts_backward", _st, [_i, _i, _vp, _i64, _vp, _i64, _vp, _i64, _u64, _u32, _u32, _i, _i, _f32, _vp, _vp]),
+    ("heph_expert_order", _st, [_i, _vp, _u64, _u32, _vp, _vp, _vp, _vp]),
+    ("heph_sample_tokens", _st, [_i, _i, _vp, _i64, _u64, _u32, _vp, _vp, _f64, _vp, _i32, _vp, _f64, _vp, _f64, _vp, _vp,
+                                 _vp]),
     ("heph_synth_fill", _st, [_vp, _vp, _u64, _u64, _i, _u64, _u64, _vp]),
     ("heph_synth_inject_row_ties", _st, [_vp, _vp, _u64, _u64, _u64, _vp]),
 ]

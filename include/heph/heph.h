@@ -472,6 +472,104 @@ heph_status heph_scan_reduce_host(heph_device *device, heph_op scan_op, int excl
 heph_status heph_reduce_full_noalloc(heph_op op, heph_dtype in_dtype, heph_dtype out_dtype,
                                      const void *in, uint64_t count, void *out, heph_stream stream);
 
+/* ------------------------------------ [EXT] language-model row operators */
+
+/* No counterparts in the reference.  Operators over the rows of a matrix in
+ * caller-owned device memory of device `ordinal`: columns are adjacent, row r
+ * starts `stride` elements after row r-1 (0 repeats a row).  They allocate
+ * nothing and need no heph_device; a NULL stream is the legacy default
+ * stream; the calling thread's current device is left as it was.  Outputs are
+ * contiguous and must not alias an input or one another.  Calls may run at
+ * the same time on any streams and may be captured into graphs.  Every sum,
+ * softmax statistic and norm is held in 32 bits or more, and no result
+ * depends on the order of atomics. */
+typedef enum heph_row_dtype {
+    HEPH_ROW_F32 = 0,
+    HEPH_ROW_BF16 = 1,
+    HEPH_ROW_F16 = 2
+} heph_row_dtype;
+
+/* Root-mean-square norm: s = x + residual (NULL: x), y = weight * s /
+ * sqrt(mean(s^2) + eps), a row of `sum` receives s.  weight: `cols` elements
+ * of the rows' type or f32, NULL for ones.  s is not rounded before the norm.
+ * A row that holds a NaN or an infinity has NaN in y where IEEE has it. */
+heph_status heph_rms_norm(int ordinal, heph_row_dtype dtype, const void *x, int64_t x_stride,
+                          const void *residual, int64_t residual_stride, const void *weight,
+                          heph_row_dtype weight_dtype, double eps, uint64_t rows, uint64_t cols,
+                          void *y, void *sum, heph_stream stream);
+/* The same with y as e4m3 values q and scales, y ~ q * scale: a scale for a
+ * row (group = 0) or for every `group` columns (a power of two >= 16, the
+ * last group may be shorter; at most 8192 groups), scale = max(max|y|,
+ * 2^-100) / 448, `scales` [rows, groups]. */
+heph_status heph_rms_norm_fp8(int ordinal, heph_row_dtype dtype, const void *x, int64_t x_stride,
+                              const void *residual, int64_t residual_stride, const void *weight,
+                              heph_row_dtype weight_dtype, double eps, uint64_t rows, uint64_t cols,
+                              uint32_t group, uint8_t *q, float *scales, void *sum, heph_stream stream);
+/* Gradient of heph_rms_norm at its sum x (or x, without a residual): dx =
+ * d(sum dy*y)/dx + dsum (NULL: 0; the gradient that reaches the sum by other
+ * ways), which is also the residual's gradient, and dweight (NULL: not
+ * wanted) in the weight's type, summed over the rows in a fixed order.  The
+ * workspace (16-byte aligned, of the size the first call tells; NULL without
+ * dweight) is free again when the call's work has run. */
+heph_status heph_rms_norm_backward_workspace(int ordinal, uint64_t rows, uint64_t cols, uint64_t *out_bytes);
+heph_status heph_rms_norm_backward(int ordinal, heph_row_dtype dtype, const void *dy, int64_t dy_stride,
+                                   const void *x, int64_t x_stride, const void *dsum, int64_t dsum_stride,
+                                   const void *weight, heph_row_dtype weight_dtype, double eps, uint64_t rows,
+                                   uint64_t cols, void *dx, void *dweight, void *workspace,
+                                   uint64_t workspace_bytes, heph_stream stream);
+
+typedef enum heph_route_score {
+    HEPH_ROUTE_SOFTMAX = 0,
+    HEPH_ROUTE_SIGMOID = 1
+} heph_route_score;
+
+/* Routes every row of `logits` to k of `experts` (<= 1024; k <= 32): scores s
+ * = softmax or sigmoid of the logits; c = s + bias (NULL: s) chooses.  With
+ * groups > 1 (equal runs of experts, <= 32 of them) a group is worth the sum
+ * of its group_top (1 or 2) largest c and only the best groups_kept groups
+ * stay.  `picks` [rows, k] receives the experts of largest c in falling order,
+ * the lowest index first among equals; `weights` their scale * s, or, renormalised,
+ * scale * s / (sum of the row's chosen s).  An expert whose logit or bias is
+ * -inf or NaN is not chosen; where none is left, the pick is -1 with weight 0. */
+heph_status heph_route_experts(int ordinal, heph_row_dtype dtype, const void *logits, int64_t stride,
+                               const float *bias, uint64_t rows, uint32_t experts, uint32_t k,
+                               heph_route_score score, uint32_t groups, uint32_t groups_kept,
+                               uint32_t group_top, int renormalize, float scale, float *weights,
+                               int32_t *picks, heph_stream stream);
+/* Gradient of the weights by the logits, the choice being constant: dlogits
+ * [rows, experts] in the logits' type, whole rows.  Picks outside [0,
+ * experts) have no part in it. */
+heph_status heph_route_experts_backward(int ordinal, heph_row_dtype dtype, const float *dweights,
+                                        int64_t dweights_stride, const void *logits, int64_t stride,
+                                        const int32_t *picks, int64_t picks_stride, uint64_t rows,
+                                        uint32_t experts, uint32_t k, heph_route_score score,
+                                        int renormalize, float scale, void *dlogits, heph_stream stream);
+
+/* The order of `count` routed pairs by expert: offsets [experts + 1] (the
+ * exclusive scan of the experts' counts), order [count] (the pairs' places,
+ * by expert and then by place; -1 past the last), slot [count] (the inverse:
+ * where a pair stands in `order`, -1 where its pick is outside [0, experts)).
+ * experts <= 1024. */
+heph_status heph_expert_order(int ordinal, const int32_t *picks, uint64_t count, uint32_t experts,
+                              int32_t *offsets, int32_t *order, int32_t *slot, heph_stream stream);
+
+/* Draws a token from every row of `logits`: w_i = exp((l_i - max l) / T).  In
+ * the order of falling l (lowest index first among equals) top_k keeps the
+ * first k (0: off), top_p of those the ones before which lies less than top_p
+ * of their mass (1: off), min_p of those the ones with w >= min_p (0: off);
+ * the first always stays.  The token is the first index whose running sum of
+ * kept w exceeds uniform[row] (in [0, 1)) times the whole; `probs` receives its
+ * share of the kept w.  T = 0 takes the first.  Each setting is one value, or
+ * a device array with one per row (NULL: the value); in an array a
+ * temperature <= 0 or NaN takes the first, and a top_k <= 0, a top_p >= 1 or NaN and
+ * a min_p <= 0 or NaN are off.  NaN logits count as -inf; a row of nothing but -inf has token -1
+ * and prob 0. */
+heph_status heph_sample_tokens(int ordinal, heph_row_dtype dtype, const void *logits, int64_t stride,
+                               uint64_t rows, uint32_t vocab, const float *uniform,
+                               const float *temperature, double temperature_all, const int32_t *top_k,
+                               int32_t top_k_all, const float *top_p, double top_p_all,
+                               const float *min_p, double min_p_all, int64_t *tokens, float *probs, heph_stream stream);
+
 #ifdef __cplusplus
 }
 #endif
