@@ -18,10 +18,29 @@ namespace cg = cooperative_groups;
 constexpr int kOrderThreads = 1024;
 constexpr int kOrderWarps = kOrderThreads / 32;
 
+constexpr int kSteps = 16;  // steps of a warp whose picks are loaded together
+
+__device__ __forceinline__ void load_picks(const int32_t *picks, uint64_t at, uint64_t end, uint32_t (&e)[kSteps]) {
+    at += threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) e[i] = at + 32 * i < end ? (uint32_t)picks[at + 32 * i] : ~0u;
+}
+
+// The lanes whose pick is this lane's, from a vote on each bit of the picks.
+// (match.any takes a turn for each different value: 41 us instead of 9 for
+// 262144 pairs of 256 experts.)
+__device__ __forceinline__ uint32_t lanes_alike(uint32_t e, bool has, int bits) {
+    uint32_t peers = __ballot_sync(kFullMask, has);
+    for (int b = 0; b < bits; ++b) {
+        const uint32_t ones = __ballot_sync(kFullMask, e >> b & 1u);
+        peers &= e >> b & 1u ? ones : ~ones;
+    }
+    return peers;
+}
+
 // One cluster sorts everything.  Block c takes the c-th part of the places,
 // warp w of it the w-th part of those, 32 adjacent places a step, so counts
-// and ranks follow the places' order and no result hangs on the order of
-// atomics (there are none).
+// and ranks follow the places' order.
 __global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(const int32_t *picks, uint32_t count, uint32_t experts,
                                                                      int32_t *offsets, int32_t *order, int32_t *slot) {
     extern __shared__ uint32_t smem[];
@@ -36,14 +55,27 @@ __global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(const int32
     const uint64_t begin = per_warp * (block * kOrderWarps + warp);
     const uint64_t end = begin + per_warp < count ? begin + per_warp : count;
     uint32_t *mine = hist + warp * experts;
+    const int bits = 32 - __clz(experts - 1);
 
     for (uint32_t i = t; i < kOrderWarps * experts; i += kOrderThreads) hist[i] = 0;
     __syncthreads();
-    for (uint64_t at = begin; at < end; at += 32) {
-        const uint32_t e = at + lane < end ? (uint32_t)picks[at + lane] : ~0u;
-        const uint32_t peers = __match_any_sync(kFullMask, e);
-        if (e < experts && (peers & ((1u << lane) - 1)) == 0) mine[e] += __popc(peers);
-        __syncwarp();
+    // The picks of kSteps steps are loaded together; the first batch (mostly
+    // the only one) stays in registers for the second walk.
+    uint32_t first[kSteps];
+    load_picks(picks, begin, end, first);
+    for (uint64_t at = begin; at < end; at += 32 * kSteps) {
+        uint32_t e[kSteps];
+        if (at == begin) {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) e[i] = first[i];
+        } else {
+            load_picks(picks, at, end, e);
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            if (at + 32 * i >= end) break;
+            if (e[i] < experts) atomicAdd(&mine[e[i]], 1u);  // a count does not depend on the order
+        }
     }
     __syncthreads();
     // Counts of the warps below, per expert.
@@ -85,20 +117,30 @@ __global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(const int32
     }
     if (block == 0 && t == 0) offsets[experts] = (int32_t)taken;
     __syncthreads();
-    for (uint64_t at = begin; at < end; at += 32) {
-        const bool in = at + lane < end;
-        const uint32_t e = in ? (uint32_t)picks[at + lane] : ~0u;
-        const uint32_t peers = __match_any_sync(kFullMask, e);
-        const uint32_t lower = peers & ((1u << lane) - 1);
-        const bool taken_up = e < experts;
-        const uint32_t place = taken_up ? mine[e] + __popc(lower) : 0;
-        __syncwarp();
-        if (taken_up) {
-            if (lower == 0) mine[e] += __popc(peers);
-            order[place] = (int32_t)(at + lane);
+    for (uint64_t at = begin; at < end; at += 32 * kSteps) {
+        uint32_t e[kSteps];
+        if (at == begin) {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) e[i] = first[i];
+        } else {
+            load_picks(picks, at, end, e);
         }
-        if (in) slot[at + lane] = taken_up ? (int32_t)place : -1;
-        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const uint64_t place = at + 32 * i + lane;
+            if (at + 32 * i >= end) break;
+            const bool has = e[i] < experts;
+            const uint32_t peers = lanes_alike(e[i], has, bits);
+            const uint32_t lower = peers & ((1u << lane) - 1);
+            const uint32_t to = has ? mine[e[i]] + __popc(lower) : 0;
+            __syncwarp();
+            if (has) {
+                if (lower == 0) mine[e[i]] += __popc(peers);
+                order[to] = (int32_t)place;
+            }
+            if (place < end) slot[place] = has ? (int32_t)to : -1;
+            __syncwarp();
+        }
     }
     for (uint64_t i = taken + (uint64_t)block * kOrderThreads + t; i < count; i += blocks * kOrderThreads) order[i] = -1;
     cluster.sync();  // no block leaves while its counts may be read

@@ -35,11 +35,11 @@ template <typename F> heph_status dispatch_row_dtype(heph_row_dtype dt, F &&f) {
 
 // An unsigned key in the order of the floats; -0 and +0 have the same key,
 // NaN has that of -inf.
-__device__ __forceinline__ uint32_t ordered_key(float v) {
-    v = v == v ? v + 0.0f : -INFINITY;
-    const uint32_t b = __float_as_uint(v);
-    return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+__device__ __forceinline__ uint32_t ordered_number(float v) {  // v is not NaN
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ uint32_t ordered_key(float v) { return ordered_number(v == v ? v : -INFINITY); }
 __device__ __forceinline__ float key_value(uint32_t key) {
     return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
 }

@@ -7,14 +7,25 @@
 //   always stays.  The token is the first index whose running sum of kept w
 //   exceeds u times the whole.
 //
-// What is kept is a threshold: all keys above one key and, by index, some of
-// those equal to it.  The threshold is found by histograms of keys (counts
-// for top-k, masses for top-p) of ever narrower ranges, with no sort.
-//
-// Masses are whole numbers, w in units of 2^-scale_bits (45 for a vocabulary
+// Masses are whole numbers, w in units of 2^-scale_bits (44 for a vocabulary
 // of 2^17), so that sums do not depend on their order: the answer is the same
 // in any batch and for any number of blocks per row.
+//
+// A row (a few hundred KB, read from memory once and then from L2) belongs to
+// a block, or to a cluster of blocks where there are few rows.  Each row takes
+// the shortest way that its settings allow:
+//   largest only    one pass for the maximum, one for its first index;
+//   top-k           a histogram of the logits tells which can be among the
+//                   first k; these (hardly more than k) are gathered and sorted
+//                   in shared memory, where the rest is prefix sums;
+//   top-p           the same with a histogram of masses;
+//   neither         the masses of the warps' parts, and a walk through one;
+//   top-k or top-p that leave over 1024  the threshold (a key, and how many of
+//                   those equal to it) by histograms of ever narrower ranges,
+//                   then as above.
 #include <cooperative_groups.h>
+
+#include <cfloat>
 
 #include "row_ops.h"
 #include "row_utils.cuh"
@@ -25,11 +36,13 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kSampleThreads = 1024;
+constexpr int kSampleThreads = 512;
 constexpr int kSampleWarps = kSampleThreads / 32;
-constexpr int kBinBits = 12;
+constexpr int kBinBits = 10;
 constexpr int kBins = 1 << kBinBits;
 constexpr int kBinsPerThread = kBins / kSampleThreads;
+constexpr int kListed = 1024;  // candidates that are sorted in shared memory
+constexpr int kEach = kListed / kSampleThreads;
 constexpr int kMaxCluster = 8;
 
 struct SampleParams {
@@ -49,16 +62,28 @@ struct Histogram {
     uint32_t low[kBins], high[kBins];  // 64-bit masses, or counts in `low`
 };
 
+// Everything that is kept: logits above `value`, and the first `ties` equal to it.
+struct Threshold {
+    float value;
+    uint32_t ties;
+};
+
 struct SampleShared {
     Histogram hist[2];
-    float max;
-    uint64_t mass;                    // this block's kept mass above the threshold
-    uint32_t ties;                    // and its number of keys equal to it
+    uint64_t list[kListed];  // candidates: not-key above index, so that they rise in the order of the choice
+    uint64_t mass[kListed];  // of the sorted candidates
+    uint64_t scan[kSampleWarps];
     uint64_t warp_mass[kSampleWarps];
     uint32_t warp_ties[kSampleWarps];
-    uint64_t scan[kSampleWarps];
+    uint64_t block_mass;  // this block's share of a sum, read by the cluster
+    uint32_t block_ties;
+    float block_max, block_sum;
+    uint32_t block_count;
+    double roots[16];
+    uint32_t listed[2];  // entries in `list`, and in `mass` where that is the second list
+    Threshold keep;
     uint32_t found_bin;
-    uint64_t found_above;
+    uint64_t found_above, found_in, kept_mass;
 };
 
 // Adds a 64-bit mass by two 32-bit atomics, whose order changes nothing.
@@ -79,157 +104,322 @@ __device__ __forceinline__ uint64_t warp_scan(uint64_t v) {  // inclusive
     return v;
 }
 
-// One row, seen by one block of its cluster: the block takes an equal part of
-// the row's 16-byte vectors, each of its warps an equal part of those, so
-// that blocks, warps, steps, lanes and elements are in the order of indices.
+// Sum of v over the threads below, and over all; two barriers.
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, SampleShared &s, uint64_t &all) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint64_t upto = warp_scan(v);
+    __syncthreads();
+    if (lane == 31) s.scan[warp] = upto;
+    __syncthreads();
+    uint64_t below = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kSampleWarps; ++w) {
+        below += w < (int)warp ? s.scan[w] : 0;
+        all += s.scan[w];
+    }
+    return below + upto - v;
+}
+
+// One row, seen by one warp: the row's 16-byte vectors are cut into equal
+// parts, so that blocks, warps, steps, lanes and elements follow the indices.
 template <typename T> struct RowPart {
     static constexpr int V = 16 / sizeof(T);
     const T *row;
-    uint32_t vocab, lead;  // lead: elements of the first vector before the row
-    uint32_t begin, end;   // vectors of this warp
+    const uint4 *vectors;  // the row's first vector, `lead` elements before it
+    uint32_t vocab, lead;
+    uint32_t begin, end;             // vectors of this warp
+    uint32_t whole_begin, whole;     // of these, the ones that lie in the row: first, and how many
 
     __device__ RowPart(const T *row_, uint32_t vocab_, uint32_t parts, uint32_t part) : row(row_), vocab(vocab_) {
         lead = (uint32_t)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
-        const uint32_t vectors = (lead + vocab + V - 1) / V;
-        const uint32_t each = ((vectors + parts - 1) / parts + 31) / 32 * 32;
-        begin = min(each * part, vectors);
-        end = min(begin + each, vectors);
+        vectors = reinterpret_cast<const uint4 *>(row - lead);
+        const uint32_t count = (lead + vocab + V - 1) / V;
+        const uint32_t each = ((count + parts - 1) / parts + 31) / 32 * 32;
+        begin = min(each * part, count);
+        end = min(begin + each, count);
+        whole_begin = begin + (begin == 0 && lead);
+        const uint32_t whole_end = min(end, (lead + vocab) / V);
+        whole = whole_end > whole_begin ? whole_end - whole_begin : 0;
     }
-    // Elements of vector q; those outside the row are NaN.
-    __device__ __forceinline__ void load(uint32_t q, float (&v)[V]) const {
-        const int64_t at = (int64_t)q * V - lead;
-        if (at >= 0 && at + V <= vocab) {
-            const auto u = *reinterpret_cast<const Pack<T, V> *>(row + at);
+    // Vector q; what is outside the part or the row is NaN.
+    __device__ __forceinline__ uint4 load(uint32_t q) const {
+        return q - whole_begin < whole ? vectors[q] : load_edge(q);
+    }
+    __device__ __noinline__ uint4 load_edge(uint32_t q) const {
+        Pack<T, V> u;
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = to_f32(u.e[j]);
-        } else {
+        for (int j = 0; j < V; ++j) {
+            const uint32_t at = q * V + j - lead;  // wraps before the row
+            u.e[j] = q < end && at < vocab ? row[at] : from_f32<T>(NAN);
+        }
+        return bitcast<uint4>(u);
+    }
+    // f(logits, index of the first) for every vector of the part; what is
+    // outside is NaN.
+    template <typename F> __device__ __forceinline__ void each(F &&f) const {
+        uint32_t q = begin + (threadIdx.x & 31);
+        uint4 a = load(q), b = load(q + 32);
+#pragma unroll 1
+        for (; q < end; q += 64) {
+            const uint4 c = load(q + 64), d = load(q + 96);
+            float u[V], v[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = at + j >= 0 && at + j < vocab ? to_f32(row[at + j]) : NAN;
+            for (int j = 0; j < V; ++j) {
+                u[j] = to_f32(bitcast<Pack<T, V>>(a).e[j]);
+                v[j] = to_f32(bitcast<Pack<T, V>>(b).e[j]);
+            }
+            f(u, q * V - lead);
+            f(v, (q + 32) * V - lead);
+            a = c;
+            b = d;
         }
     }
-    // f(logit) for every element of the warp's part.
-    template <typename F> __device__ __forceinline__ void each(F &&f) const {
-        for (uint32_t q = begin + (threadIdx.x & 31); q < end; q += 32) {
-            float v[V];
-            load(q, v);
-#pragma unroll
-            for (int j = 0; j < V; ++j) f(v[j]);
+    // f(logit, logit) for all elements, two at a time: for work so long that it
+    // is written out once only (the instructions come from the cache too).
+    template <typename F> __device__ __forceinline__ void each_two(F &&f) const {
+        uint32_t q = begin + (threadIdx.x & 31);
+        uint4 a = load(q), b = load(q + 32);
+#pragma unroll 1
+        for (; q < end; q += 32) {
+            const uint4 c = load(q + 64);
+#pragma unroll 1
+            for (int i = 0; i < V / 2; ++i) {
+                if constexpr (sizeof(T) == 4) {
+                    f(__uint_as_float(a.x), __uint_as_float(a.y));
+                    a.x = a.z;
+                    a.y = a.w;
+                } else {
+                    const auto two = bitcast<Pack<T, 2>>(a.x);
+                    f(to_f32(two.e[0]), to_f32(two.e[1]));
+                    a.x = a.y;
+                    a.y = a.z;
+                    a.z = a.w;
+                }
+            }
+            a = b;
+            b = c;
         }
     }
 };
+
+// 2^(i / 16) by table, 2^(r / 16) for |r| <= 1/2 by the polynomial through the
+// six Chebyshev nodes there, its constant being made 1: within 1e-14 together.
+// (A table of 16 is 128 bytes of shared memory, one round of its banks.)
+__constant__ double kRoots[16] = {
+    0x1.0000000000000p+0, 0x1.0b5586cf9890fp+0, 0x1.172b83c7d517bp+0, 0x1.2387a6e756238p+0,
+    0x1.306fe0a31b715p+0, 0x1.3dea64c123422p+0, 0x1.4bfdad5362a27p+0, 0x1.5ab07dd485429p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.7a11473eb0187p+0, 0x1.8ace5422aa0dbp+0, 0x1.9c49182a3f090p+0,
+    0x1.ae89f995ad3adp+0, 0x1.c199bdd85529cp+0, 0x1.d5818dcfba487p+0, 0x1.ea4afa2a490dap+0};
+__constant__ double kExp2[6] = {0x1.0000000000000p+0,  0x1.62e42fefa39f3p-5,  0x1.ebfbdff555824p-11,
+                                0x1.c6b08d6f2a289p-17, 0x1.3b2c9b8a6caeap-23, 0x1.5d897e525c216p-30};
 
 struct Weigher {
-    float max;
-    double inverse_t, unit, least;  // unit = 2^scale_bits; least: min_p
-    __device__ __forceinline__ double weight(float l) const {
-        return l == max ? 1.0 : exp(((double)l - (double)max) * inverse_t);
+    float max, floor;  // floor: a lower logit has no mass
+    float top, slope32;  // max, or the largest finite number; slope in 32 bits
+    double slope;        // 16 log2(e) / T
+    int scale_bits;
+    const double *roots;  // kRoots in shared memory
+
+    __device__ Weigher(float max_, double t, int scale_bits_, const double *roots_)
+        : max(max_), scale_bits(scale_bits_), roots(roots_) {
+        top = fminf(max, FLT_MAX);
+        slope = 16 * 1.4426950408889634 / t;
+        slope32 = (float)slope;
+        // Below half a unit; and no -inf, whatever the temperature.
+        floor = fmaxf(__double2float_rd((double)max - (scale_bits + 1.5) * 0.6931471805599453 * t), -FLT_MAX);
     }
-    __device__ __forceinline__ uint64_t mass(float l) const { return __double2ull_rn(weight(l) * unit); }
-    // The mass, or none where min-p drops it.
-    __device__ __forceinline__ uint64_t kept_mass(float l) const {
-        const double w = weight(l);
-        return w >= least ? __double2ull_rn(w * unit) : 0;
+    // exp((l - max) / T) 2^scale_bits, rounded, for l >= floor (else anything);
+    // a unit is at least 2^-45 of the maximum's mass, which is 2^scale_bits.
+    __device__ __forceinline__ uint64_t mass(float l) const {
+        l = fminf(l, FLT_MAX);  // an infinity is equal to itself
+        // n = 16 log2(w) rounded, in the low bits of `at`.
+        const float magic = 0x1.8p23f, at = (l - top) * slope32 + magic;
+        const uint32_t n = __float_as_uint(at);
+        const double r = fma((double)l - (double)top, slope, -(double)(at - magic));
+        double p = kExp2[5];
+#pragma unroll
+        for (int i = 4; i >= 0; --i) p = fma(p, r, kExp2[i]);
+        p *= roots[n & 15];
+        // (n >> 4) + scale_bits more in the exponent; magic's own bits are shifted out.
+        const double w = __hiloint2double(__double2hiint(p) + ((n & ~15u) << 16) + (scale_bits << 20), __double2loint(p));
+        return (uint64_t)__double_as_longlong(w + 0x1p52) & 0xfffffffffffffull;
+    }
+    // The same unrounded, for the answer's probability.
+    __device__ double share(float l, uint64_t all) const {
+        const double w = l == max ? 1.0 : exp2(((double)l - (double)max) * (slope / 16));
+        return ldexp(w, scale_bits) / (double)all;
+    }
+    __device__ __forceinline__ uint64_t mass_or_none(float l) const { return l >= floor ? mass(l) : 0; }
+    // Of two at once, whose long chains of operations overlap.
+    __device__ __forceinline__ void masses(float a, float b, float from, uint64_t &x, uint64_t &y) const {
+        x = y = 0;
+        if (a >= from || b >= from) {
+            const uint64_t u = mass(a), v = mass(b);
+            x = a >= from ? u : 0;
+            y = b >= from ? v : 0;
+        }
     }
 };
 
-// Everything that is kept: keys above `key`, and the first `ties` equal to it.
-struct Threshold {
-    uint32_t key, ties;
+// Which of 1024 equal steps below the maximum a logit is nearest to; the last
+// takes all that is further down.  Falls monotonically in l.
+struct Steps {
+    float top, width;  // top is finite: +inf is in step 0 too
+    float per_unit;
+    __device__ Steps(const Weigher &weigh, float window) : top(weigh.top), width(window / kBins), per_unit(kBins / window) {}
+    __device__ __forceinline__ uint32_t bin(float l) const {
+        return __float_as_uint(fminf((top - l) * per_unit, (float)(kBins - 1)) + 0x1p23f) & (kBins - 1);
+    }
+    // No logit of step `bin` is above the one or below the other (a margin
+    // covers the roundings of the step's number).
+    __device__ float above(uint32_t bin) const {
+        return bin ? __double2float_ru((double)top - (bin - 0.5) * width * (1.0 - 1e-6)) : INFINITY;
+    }
+    __device__ float below(uint32_t bin) const {
+        return bin < kBins - 1 ? __double2float_rd((double)top - (bin + 0.5) * width * (1.0 + 1e-6)) : -INFINITY;
+    }
+};
+
+template <int V> __device__ __forceinline__ float largest(const float (&v)[V]) {  // fmaxf passes NaN over
+    float m = v[0];
+#pragma unroll
+    for (int j = 1; j < V; ++j) m = fmaxf(m, v[j]);
+    return m;
+}
+
+// Sum of what `of` is in the blocks below `upto` of the cluster, by every warp.
+template <typename N> __device__ __forceinline__ N sum_over_blocks(const N &of, uint32_t upto) {
+    const uint32_t lane = threadIdx.x & 31;
+    const cg::cluster_group cluster = cg::this_cluster();
+    N v = 0;
+    if (lane < upto) v = *cluster.map_shared_rank(&of, lane);
+    return warp_fold<N, OP_SUM>(v);
+}
+
+__device__ __noinline__ void mass_to_bin(const Weigher &weigh, Histogram &h, uint32_t bin, float l) {
+    const uint64_t mass = weigh.mass_or_none(l);
+    if (mass) add_mass(h, bin, mass);
+}
+
+__device__ __forceinline__ void clear(Histogram &h) {
+    for (int i = threadIdx.x; i < kBins; i += kSampleThreads) h.low[i] = h.high[i] = 0;
+    __syncthreads();
+}
+
+// After a cluster barrier: the sums of the blocks' histograms, the first bin
+// at which `before` plus the running sum reaches `wanted(all)` (kBins: none),
+// what it holds, and the sum before it; the same for every block.
+template <bool MASS, typename Wanted>
+__device__ uint32_t find_bin(Histogram &h, SampleShared &s, uint64_t before, Wanted &&wanted) {
+    const cg::cluster_group cluster = cg::this_cluster();
+    using Bins = Pack<uint32_t, kBinsPerThread>;
+    const uint32_t t = threadIdx.x;
+    uint64_t bins[kBinsPerThread] = {}, sum = 0, all;
+    Bins lo[kMaxCluster] = {}, hi[kMaxCluster] = {};
+#pragma unroll
+    for (uint32_t b = 0; b < kMaxCluster; ++b) {
+        if (b < cluster.num_blocks()) {
+            const Histogram *o = cluster.map_shared_rank(&h, b);
+            lo[b] = *reinterpret_cast<const Bins *>(&o->low[t * kBinsPerThread]);
+            if (MASS) hi[b] = *reinterpret_cast<const Bins *>(&o->high[t * kBinsPerThread]);
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < kMaxCluster; ++b)
+#pragma unroll
+        for (int i = 0; i < kBinsPerThread; ++i) bins[i] += (uint64_t)hi[b].e[i] << 32 | lo[b].e[i];
+#pragma unroll
+    for (int i = 0; i < kBinsPerThread; ++i) sum += bins[i];
+    if (t == 0) s.found_bin = kBins;
+    uint64_t run = before + block_scan(sum, s, all);
+    const uint64_t goal = wanted(all);
+#pragma unroll
+    for (int i = 0; i < kBinsPerThread; ++i) {
+        if (run < goal && run + bins[i] >= goal) {
+            s.found_bin = t * kBinsPerThread + i;
+            s.found_above = run;
+            s.found_in = bins[i];
+        }
+        run += bins[i];
+    }
+    __syncthreads();
+    return s.found_bin;
+}
+
+// The step of the logit in which a search is known to end.
+struct Located {
+    uint32_t bin = kBins;  // not known
+    uint64_t above = 0, wanted = 0;
 };
 
 struct Narrowed {
-    uint32_t key;
-    uint64_t above;  // count or mass of the keys above `key`
+    uint32_t key;    // 0: the row's keys above the floor do not reach it
+    uint64_t above;  // count or mass of the keys above `key`, or of all
     uint64_t wanted;
 };
 
-// The largest key whose keys-at-or-above hold at least wanted = need(total)
-// (counts, or with MASS masses), among the row's keys above `floor`, of which
-// `total` is the whole; key = floor where these do not reach it.  First by 4096 equal steps of the logit below the
-// maximum (a window of `window`; the last bin takes the rest), which spreads
-// any scale of logits; then, within one bin, by steps of the key.
+// The largest key such that the keys at or above it hold at least wanted =
+// need(total) (a count, or with MASS a mass), among the row's logits above
+// `floor`, of which `total` is the whole.  First by steps of the logit below
+// the maximum, which spreads any scale of logits; then, within one of them,
+// by steps of the key.
 template <bool MASS, typename T, typename Need>
-__device__ Narrowed narrow(const RowPart<T> &part, const Weigher &weigh, SampleShared &s, int &turn, uint32_t floor,
-                           float window, Need &&need) {
+__device__ Narrowed narrow(const RowPart<T> &part, const Weigher &weigh, SampleShared &s, int &turn, float floor,
+                           float window, const Located &start, Need &&need) {
     const cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const float max = weigh.max, steps = kBins / window;
-    auto linear_bin = [&](float l) -> uint32_t {
-        return l == max ? 0 : (uint32_t)fminf((max - l) * steps, (float)(kBins - 1));
+    const Steps steps(weigh, window);
+    Narrowed got{0, start.above, start.wanted};
+    uint32_t first = start.bin, high = ordered_key(weigh.max), low = 1;
+    int shift = -1;  // -1: steps of the logit
+    // The keys that step `first` may have; which of them belong is decided by
+    // their step's number.
+    auto enter_step = [&] {
+        high = ::min(high, ordered_key(steps.above(first)));
+        low = ::max(low, ordered_key(steps.below(first)));
     };
-    Narrowed got{floor, 0, 0};
-    uint32_t first = 0, high = ordered_key(max), low = floor + 1;
-    int shift = -1;  // -1: the linear bins
+    if (first < kBins) {
+        enter_step();
+        shift = ::max(0, 32 - __clz(high - low) - kBinBits);
+    }
     for (;;) {
         Histogram &h = s.hist[turn];
         turn ^= 1;
-        for (int i = t; i < kBins; i += kSampleThreads) h.low[i] = h.high[i] = 0;
-        __syncthreads();
-        part.each([&](float l) {
-            if (!(l == l)) return;
-            const uint32_t key = ordered_key(l);
-            if (key < low || key > high) return;
-            uint32_t bin = linear_bin(l);
-            if (shift >= 0) {
-                if (bin != first) return;
-                bin = (high - key) >> shift;
-            }
-            if constexpr (MASS) {
-                const uint64_t mass = weigh.mass(l);
-                if (mass) add_mass(h, bin, mass);
-            } else {
-                atomicAdd(&h.low[bin], 1u);
+        clear(h);
+        // Logits that may be counted now; all others are passed over.
+        const float from = shift < 0 ? floor : key_value(low), upto = shift < 0 ? INFINITY : key_value(high);
+        part.each([&](const float(&v)[RowPart<T>::V], uint32_t) {
+            if (!(largest(v) >= from)) return;
+#pragma unroll
+            for (int j = 0; j < RowPart<T>::V; ++j) {
+                const float l = v[j];
+                if (!(l >= from && l <= upto && l > floor)) continue;
+                uint32_t bin = steps.bin(l);
+                if (shift >= 0) {
+                    if (bin != first) continue;
+                    bin = (high - ordered_number(l)) >> shift;
+                }
+                if constexpr (MASS) mass_to_bin(weigh, h, bin, l);
+                else atomicAdd(&h.low[bin], 1u);
             }
         });
         cluster.sync();
-        // Every block of the cluster sums all their histograms and finds the
-        // bin by itself.  The other histogram is cleared after the next
-        // barrier at the earliest, when nobody reads this one.
-        uint64_t bins[kBinsPerThread], sum = 0;
-#pragma unroll
-        for (int i = 0; i < kBinsPerThread; ++i) bins[i] = 0;
-        for (uint32_t b = 0; b < cluster.num_blocks(); ++b) {
-            const Histogram *o = cluster.map_shared_rank(&h, b);
-            const Pack<uint32_t, kBinsPerThread> lo = *reinterpret_cast<const Pack<uint32_t, kBinsPerThread> *>(&o->low[t * kBinsPerThread]);
-            const Pack<uint32_t, kBinsPerThread> hi = *reinterpret_cast<const Pack<uint32_t, kBinsPerThread> *>(&o->high[t * kBinsPerThread]);
-#pragma unroll
-            for (int i = 0; i < kBinsPerThread; ++i) bins[i] += (uint64_t)hi.e[i] << 32 | lo.e[i];
-        }
-#pragma unroll
-        for (int i = 0; i < kBinsPerThread; ++i) sum += bins[i];
-        uint64_t upto = warp_scan(sum);
-        if (lane == 31) s.scan[warp] = upto;
-        if (t == 0) s.found_bin = kBins;
-        __syncthreads();
-        uint64_t below = 0, all = 0;
-        for (int w = 0; w < kSampleWarps; ++w) {
-            below += w < (int)warp ? s.scan[w] : 0;
-            all += s.scan[w];
-        }
-        if (shift < 0) got.wanted = need(all);
-        uint64_t run = got.above + below + upto - sum;
-#pragma unroll
-        for (int i = 0; i < kBinsPerThread; ++i) {
-            if (run < got.wanted && run + bins[i] >= got.wanted) {
-                s.found_bin = t * kBinsPerThread + i;
-                s.found_above = run;
-            }
-            run += bins[i];
-        }
-        __syncthreads();
-        const uint32_t bin = s.found_bin;
-        if (bin == kBins) {  // these keys do not reach it
-            got.above = all;
+        // The other histogram is cleared next, after this barrier, when no
+        // block reads it any more.
+        uint64_t total = 0;
+        const uint32_t bin = find_bin<MASS>(h, s, got.above, [&](uint64_t all) {
+            total = all;
+            if (shift < 0) got.wanted = need(all);
+            return got.wanted;
+        });
+        if (bin == kBins) {
+            got.above = total;
             return got;
         }
         got.above = s.found_above;
         if (shift < 0) {
-            // The keys of linear bin `bin`, with a margin for the rounding of
-            // the bin's number; which of them belong is decided by that number.
             first = bin;
-            const double width = (double)window / kBins, margin = 1e-6;
-            if (bin) high = min(high, ordered_key(__double2float_ru((double)max - bin * width * (1.0 - margin))));
-            if (bin < kBins - 1) low = ::max(low, ordered_key(__double2float_rd((double)max - (bin + 1) * width * (1.0 + margin))));
+            enter_step();
         } else {
             high -= bin << shift;
             low = ::max(low, high - ((1u << shift) - 1));
@@ -242,28 +432,195 @@ __device__ Narrowed narrow(const RowPart<T> &part, const Weigher &weigh, SampleS
     }
 }
 
+// Sorts `size` (a power of two) numbers upwards; a small list by one warp.
+__device__ void sort_list(uint64_t *list, uint32_t size) {
+    const uint32_t warp = threadIdx.x >> 5;
+    const bool small = size <= 64;
+    if (!small || warp == 0) {
+        for (uint32_t run = 2; run <= size; run *= 2) {
+            for (uint32_t d = run / 2; d > 0; d /= 2) {
+                for (uint32_t i = threadIdx.x; i < size / 2; i += kSampleThreads) {
+                    const uint32_t a = 2 * i - (i & (d - 1)), b = a + d;
+                    const uint64_t x = list[a], y = list[b];
+                    if ((x > y) == ((a & run) == 0)) {
+                        list[a] = y;
+                        list[b] = x;
+                    }
+                }
+                if (small) __syncwarp();
+                else __syncthreads();
+            }
+        }
+    }
+    __syncthreads();
+}
+
+__device__ __forceinline__ uint32_t power_from(uint32_t n) { return n <= 2 ? 2 : 1u << (32 - __clz(n - 1)); }
+
+__device__ __forceinline__ uint64_t part_of(uint64_t all, double p) {  // ceil(p all), from 1 to all
+    const double part = ceil((double)all * (p > 0.0 ? p : 0.0));
+    return part < 1.0 ? 1 : ::min((uint64_t)part, all);
+}
+__device__ __forceinline__ uint64_t point_of(uint64_t all, float u) {  // floor(u all), below all
+    return ::min((uint64_t)((u > 0.0f ? (double)fminf(u, 1.0f) : 0.0) * (double)all), all - 1);
+}
+
+// Block 0 gathers the cluster's lists (which = 1: the second) in s.list; its
+// length.  Warp b fetches block b's.
+__device__ uint32_t collect(SampleShared &s, int which) {
+    const cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t warp = threadIdx.x >> 5, blocks = cluster.num_blocks();
+    if (cluster.block_rank() == 0 && warp < blocks && (warp || which)) {
+        const uint32_t to = sum_over_blocks(s.listed[which], warp);
+        const SampleShared *o = cluster.map_shared_rank(&s, warp);
+        const uint64_t *list = which ? o->mass : o->list;
+        for (uint32_t i = threadIdx.x & 31; i < o->listed[which]; i += 32) s.list[to + i] = list[i];
+    }
+    return sum_over_blocks(s.listed[which], blocks);
+}
+
+// s.list sorted upwards, n entries and padding; this thread's kEach of them
+// (0 past n).
+__device__ void sorted_entries(SampleShared &s, uint32_t n, uint64_t (&entry)[kEach]) {
+    const uint32_t t = threadIdx.x, size = power_from(n);
+    for (uint32_t i = n + t; i < size; i += kSampleThreads) s.list[i] = ~0ull;
+    __syncthreads();
+    sort_list(s.list, size);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) entry[i] = t * kEach + i < n ? s.list[t * kEach + i] : 0;
+}
+
+__device__ __forceinline__ float entry_logit(uint64_t entry) { return key_value(~(uint32_t)(entry >> 32)); }
+
+// The threshold that is known to lie among the n entries of s.list, all there
+// are of their step of the logit.  One block.
+__device__ void threshold_from_list(const Weigher &weigh, SampleShared &s, uint32_t n, bool count, const Located &located) {
+    uint64_t entry[kEach], size[kEach], sum = 0, all;
+    sorted_entries(s, n, entry);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        size[i] = threadIdx.x * kEach + i >= n ? 0 : count ? 1 : weigh.mass_or_none(entry_logit(entry[i]));
+        sum += size[i];
+    }
+    uint64_t run = located.above + block_scan(sum, s, all);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        if (run < located.wanted && run + size[i] >= located.wanted) {
+            // The last that is kept; the ones equal to it stand before it.
+            const uint32_t r = threadIdx.x * kEach + i;
+            uint32_t first = r;
+            while (first > 0 && s.list[first - 1] >> 32 == entry[i] >> 32) --first;
+            s.keep = {entry_logit(entry[i]), r - first + 1};
+        }
+        run += size[i];
+    }
+}
+
+// Draws from the n candidates in s.list, the row's first n (or more, in no
+// order): the first k of them, of these the top-p of `whole` mass (0: of their
+// own), of these those of mass >= least.  One block.
 template <typename T>
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_constant__ SampleParams p) {
-    extern __shared__ __align__(16) unsigned char raw[];
-    SampleShared &s = *reinterpret_cast<SampleShared *>(raw);
+__device__ void draw_from_list(const T *row, const Weigher &weigh, SampleShared &s, uint32_t n, uint32_t k, double top_p, uint64_t whole,
+                               uint64_t least, float u, int64_t *token, float *prob) {
+    const uint32_t t = threadIdx.x, of = min(n, k);
+    uint64_t mass[kEach], entry[kEach], sum = 0, all;
+    sorted_entries(s, n, entry);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        mass[i] = t * kEach + i < of ? weigh.mass_or_none(entry_logit(entry[i])) : 0;
+        sum += mass[i];
+    }
+    uint64_t run = block_scan(sum, s, all);
+    const uint64_t wanted = top_p < 1.0 ? part_of(whole ? whole : all, top_p) : ~0ull;
+    bool keep[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const uint32_t r = t * kEach + i;
+        keep[i] = r < of && run < wanted && (mass[i] >= least || r == 0);
+        run += mass[i];
+        if (r < kListed) s.mass[r] = mass[i];
+    }
+    uint32_t kept = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) kept += __syncthreads_count(keep[i]);
+    // The kept ones by index, and their running sum.
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const uint32_t r = t * kEach + i;
+        if (r < kept) s.list[r] = entry[i] << 32 | r;
+    }
+    __syncthreads();
+    sorted_entries(s, kept, entry);
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        mass[i] = t * kEach + i < kept ? s.mass[(uint32_t)entry[i]] : 0;
+        sum += mass[i];
+    }
+    run = block_scan(sum, s, all);
+    const uint64_t point = point_of(all, u);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        if (point >= run && point < run + mass[i]) {
+            *token = (int64_t)(entry[i] >> 32);
+            *prob = (float)weigh.share(to_f32(row[entry[i] >> 32]), all);
+        }
+        run += mass[i];
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_constant__ SampleParams p) {
+    __shared__ SampleShared s;
     const cg::cluster_group cluster = cg::this_cluster();
     const uint32_t blocks = cluster.num_blocks(), block = cluster.block_rank();
     const uint32_t row = blockIdx.x / blocks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const RowPart<T> part(static_cast<const T *>(p.logits) + row * p.stride, p.vocab, blocks * kSampleWarps,
                           block * kSampleWarps + warp);
+    const double t = p.temperature ? p.temperature[row] : p.temperature_all;
+    const int32_t k = p.top_k ? p.top_k[row] : p.top_k_all;
+    const double top_p = p.top_p ? p.top_p[row] : p.top_p_all;
+    const double min_p = p.min_p ? p.min_p[row] : p.min_p_all;
+    const float u = p.uniform[row];
+    const bool greedy = !(t > 0.0) || k == 1;
+    const bool by_count = !greedy && k > 0 && (uint32_t)k < p.vocab, by_mass = !greedy && top_p < 1.0;
 
-    float max = -INFINITY;
-    part.each([&](float l) { max = fmaxf(max, l); });  // fmaxf passes NaN over
+    // The maximum, and for top-k the mean, which tells the logits' scale.
+    float max = -INFINITY, sum = 0.0f;
+    uint32_t count = 0;
+    part.each([&](const float(&v)[RowPart<T>::V], uint32_t) {
+        max = fmaxf(max, largest(v));
+        if (fabsf(v[0]) < 1e4f) {  // of every V-th; no masks
+            sum += v[0];
+            ++count;
+        }
+    });
     max = warp_max(max);
-    if (lane == 0) s.warp_mass[warp] = __float_as_uint(max);
+    sum = warp_sum(sum);
+    count = warp_fold<uint32_t, OP_SUM>(count);
+    if (lane == 0) {
+        s.warp_mass[warp] = (uint64_t)__float_as_uint(max) << 32 | __float_as_uint(sum);
+        s.warp_ties[warp] = count;
+    }
+    if (threadIdx.x < 2) s.listed[threadIdx.x] = 0;
+    if (threadIdx.x < 16) s.roots[threadIdx.x] = kRoots[threadIdx.x];
     __syncthreads();
     if (warp == 0) {
-        max = warp_max(__uint_as_float((uint32_t)s.warp_mass[lane]));
-        if (lane == 0) s.max = max;
+        const bool has = lane < kSampleWarps;
+        const uint64_t both = has ? s.warp_mass[lane] : 0;
+        max = warp_max(has ? __uint_as_float((uint32_t)(both >> 32)) : -INFINITY);
+        sum = warp_sum(has ? __uint_as_float((uint32_t)both) : 0.0f);
+        count = warp_fold<uint32_t, OP_SUM>(has ? s.warp_ties[lane] : 0);
+        if (lane == 0) {
+            s.block_max = max;
+            s.block_sum = sum;
+            s.block_count = count;
+        }
     }
     cluster.sync();
-    max = -INFINITY;
-    for (uint32_t b = 0; b < blocks; ++b) max = fmaxf(max, *cluster.map_shared_rank(&s.max, b));
+    max = warp_max(lane < blocks ? *cluster.map_shared_rank(&s.block_max, lane) : -INFINITY);
+    sum = sum_over_blocks(s.block_sum, blocks);
+    count = sum_over_blocks(s.block_count, blocks);
     if (max == -INFINITY) {  // nothing to choose from
         if (block == 0 && threadIdx.x == 0) {
             p.tokens[row] = -1;
@@ -272,47 +629,169 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
         cluster.sync();
         return;
     }
-
-    const double t = p.temperature ? p.temperature[row] : p.temperature_all;
-    const int32_t k = p.top_k ? p.top_k[row] : p.top_k_all;
-    const double top_p = p.top_p ? p.top_p[row] : p.top_p_all;
-    const double min_p = p.min_p ? p.min_p[row] : p.min_p_all;
-    const bool greedy = !(t > 0.0) || k == 1;
-    const Weigher weigh{max, greedy ? 1.0 : 1.0 / t, ldexp(1.0, p.scale_bits), min_p > 0.0 ? fmin(min_p, 1.0) : 0.0};
-
-    Threshold keep{0, 0};  // no key is 0: everything
-    int turn = 0;
     if (greedy) {
-        keep = {ordered_key(max), 1};
-    } else {
-        if (k > 0 && (uint32_t)k < p.vocab) {
-            const Narrowed n = narrow<false>(part, weigh, s, turn, 0, 16.0f, [&](uint64_t) { return (uint64_t)k; });
-            if (n.key) keep = {n.key, (uint32_t)(k - n.above)};
+        uint32_t first = ~0u;
+        part.each([&](const float(&v)[RowPart<T>::V], uint32_t index) {
+#pragma unroll
+            for (int j = 0; j < RowPart<T>::V; ++j)
+                if (v[j] == max) first = min(first, index + j);
+        });
+        first = warp_fold<uint32_t, OP_MIN>(first);
+        if (lane == 0) s.warp_ties[warp] = first;
+        __syncthreads();
+        if (warp == 0) {
+            first = warp_fold<uint32_t, OP_MIN>(lane < kSampleWarps ? s.warp_ties[lane] : ~0u);
+            if (lane == 0) s.block_ties = first;
         }
-        if (top_p < 1.0) {
-            const uint64_t tie = keep.ties ? weigh.mass(key_value(keep.key)) : 0;
-            const float window = (float)fmin(fmax(32.0 * t, 0x1p-10), 0x1p10);
-            const Narrowed n = narrow<true>(part, weigh, s, turn, keep.key, window, [&](uint64_t above) -> uint64_t {
-                const uint64_t all = above + keep.ties * tie;
-                const double part_of = ceil((double)all * (top_p > 0.0 ? top_p : 0.0));
-                return part_of < 1.0 ? 1 : ::min((uint64_t)part_of, all);
+        cluster.sync();
+        if (block == 0 && threadIdx.x == 0) {
+            for (uint32_t b = 1; b < blocks; ++b) first = min(first, *cluster.map_shared_rank(&s.block_ties, b));
+            p.tokens[row] = first;
+            p.probs[row] = 1.0f;
+        }
+        cluster.sync();
+        return;
+    }
+
+    const Weigher weigh(max, t, p.scale_bits, s.roots);
+    const double least_w = min_p > 0.0 ? fmin(min_p, 1.0) : 0.0;
+    const uint64_t least = (uint64_t)ceil(least_w * (double)(1ull << p.scale_bits));
+    // top-k: the distance from the mean to the maximum covers every k below
+    // half of the vocabulary, and three quarters of it a k below an eighth (of
+    // normal logits; others are found too, the longer way).  top-p: what is left below the window is less
+    // than 1 - p of the mass, were it all as heavy as its upper end.
+    const float spread = (count && max < 1e4f ? max - sum / count : 16.0f) * ((uint32_t)k < p.vocab / 8 ? 0.75f : 1.0f);
+    const float count_window = fminf(fmaxf(spread, 0x1p-10f), 0x1p10f);
+    const float mass_window =
+        fminf(fmaxf((float)t * (__logf((float)p.vocab / fmaxf((float)(1.0 - top_p), 1e-6f)) + 0.01f), 0x1p-10f), 0x1p10f);
+    int turn = 0;
+    Located located;
+    Threshold keep{-INFINITY, 0};
+    bool found = false;
+
+    if (by_count || by_mass) {
+        Histogram &h = s.hist[turn];
+        uint32_t last = kBins - 1;
+        bool fits = p.vocab <= kListed;  // all that is kept may fit a list
+        uint64_t whole = 0;
+        const Steps steps(weigh, by_count ? count_window : mass_window);
+        const float edge = steps.top - (by_count ? count_window : mass_window);
+        if (!fits) {
+            turn ^= 1;
+            clear(h);
+        }
+        if (fits) {
+            // All of it is listed.
+        } else if (by_count) {
+            part.each([&](const float(&v)[RowPart<T>::V], uint32_t) {
+                if (!(largest(v) >= edge)) return;
+#pragma unroll
+                for (int j = 0; j < RowPart<T>::V; ++j)
+                    if (v[j] >= edge) atomicAdd(&h.low[steps.bin(v[j])], 1u);
             });
-            const uint64_t left = n.wanted - n.above;  // > 0, to be filled by keys equal to n.key
-            const uint64_t each = n.key == keep.key ? tie : weigh.mass(key_value(n.key));
-            keep = {n.key, each ? (uint32_t)((left + each - 1) / each) : keep.ties};
+            cluster.sync();
+            last = find_bin<false>(h, s, 0, [&](uint64_t) { return (uint64_t)k; });
+            if (last < kBins - 1) located = {last, s.found_above, (uint64_t)k};
+            fits = located.bin < kBins && s.found_above + s.found_in <= kListed;
+        } else {
+            uint64_t mass = 0;
+            part.each_two([&](float a, float b) {
+                uint64_t x, y;
+                weigh.masses(a, b, weigh.floor, x, y);
+                mass += x + y;
+                if (a >= edge) add_mass(h, steps.bin(a), x);
+                if (b >= edge) add_mass(h, steps.bin(b), y);
+            });
+            uint64_t mine;
+            block_scan(mass, s, mine);
+            if (threadIdx.x == 0) s.block_mass = mine;
+            cluster.sync();
+            whole = (uint64_t)sum_over_blocks((int64_t &)s.block_mass, blocks);
+            last = find_bin<true>(h, s, 0, [&](uint64_t) { return part_of(whole, top_p); });
+            fits = last < kBins - 1;
+            if (fits) located = {last, s.found_above, part_of(whole, top_p)};
+        }
+        if (fits || located.bin < kBins) {
+            // Two lists: of all that may be kept, and of the last step alone.
+            const float from = steps.below(last);
+            part.each([&](const float(&v)[RowPart<T>::V], uint32_t index) {
+                if (!(largest(v) >= from)) return;
+#pragma unroll
+                for (int j = 0; j < RowPart<T>::V; ++j) {
+                    if (!(v[j] >= from)) continue;
+                    const uint32_t bin = steps.bin(v[j]);
+                    const uint64_t entry = (uint64_t)~ordered_number(v[j]) << 32 | (index + j);
+                    // (Past its end the list is of no use, and a common counter slow.)
+                    if (fits && bin <= last && *(volatile uint32_t *)&s.listed[0] <= kListed) {
+                        const uint32_t at = atomicAdd(&s.listed[0], 1u);
+                        if (at < kListed) s.list[at] = entry;
+                    }
+                    if (bin == last) {
+                        const uint32_t at = atomicAdd(&s.listed[1], 1u);
+                        if (at < kListed) s.mass[at] = entry;
+                    }
+                }
+            });
+            cluster.sync();
+            if (fits && sum_over_blocks(s.listed[0], blocks) <= kListed) {
+                const uint32_t n = collect(s, 0);
+                cluster.sync();
+                if (block == 0)
+                    draw_from_list(part.row, weigh, s, n, by_count ? k : n, top_p, whole, least, u, p.tokens + row, p.probs + row);
+                return;
+            }
+            if (sum_over_blocks(s.listed[1], blocks) <= kListed) {
+                const uint32_t n = collect(s, 1);
+                if (block == 0) threshold_from_list(weigh, s, n, by_count, located);
+                cluster.sync();
+                keep = *cluster.map_shared_rank(&s.keep, 0);
+                found = true;
+            }
         }
     }
 
+    // The threshold, where top-k or top-p have it left to be found.
+    if (by_count && !found) {
+        const Narrowed n = narrow<false>(part, weigh, s, turn, -INFINITY, count_window, located, [&](uint64_t) { return (uint64_t)k; });
+        if (n.key) keep = {key_value(n.key), (uint32_t)(k - n.above)};
+    }
+    if (by_mass && (by_count || !found)) {
+        const uint64_t tie = keep.ties ? weigh.mass_or_none(keep.value) : 0;
+        const Narrowed n = narrow<true>(part, weigh, s, turn, keep.value, mass_window, by_count ? Located{} : located,
+                                        [&](uint64_t above) { return part_of(above + keep.ties * tie, top_p); });
+        // What is left to be filled by logits equal to the key's.
+        const uint64_t left = n.wanted - n.above, each = n.key ? weigh.mass_or_none(key_value(n.key)) : tie;
+        const uint32_t ties = each ? (uint32_t)((left + each - 1) / each) : 0;
+        keep = {n.key ? key_value(n.key) : keep.value, ties};
+    }
+
     // Kept mass and ties, per warp, block and row.
-    const uint64_t tie = keep.ties ? weigh.kept_mass(key_value(keep.key)) : 0;
+    float from = weigh.floor;  // no lower logit is kept
+    if (least_w > 0.0) from = fmaxf(from, __double2float_rd((double)max + t * (log(least_w) - 1e-9)));
+    if (keep.value >= from) from = keep.value < INFINITY ? nextafterf(keep.value, INFINITY) : NAN;  // NAN: none is above
+    auto kept_masses = [&](float a, float b, uint64_t &x, uint64_t &y) {
+        weigh.masses(a, b, from, x, y);
+        x = x >= least ? x : 0;
+        y = y >= least ? y : 0;
+    };
+    uint64_t tie = keep.ties ? weigh.mass_or_none(keep.value) : 0;
+    if (tie < least) tie = 0;
     uint64_t mass = 0;
     uint32_t ties = 0;
-    part.each([&](float l) {
-        if (!(l == l)) return;
-        const uint32_t key = ordered_key(l);
-        if (key > keep.key) mass += weigh.kept_mass(l);
-        ties += key == keep.key;
-    });
+    if (keep.ties == 0 && least == 0) {
+        part.each_two([&](float a, float b) {
+            uint64_t x, y;
+            weigh.masses(a, b, from, x, y);
+            mass += x + y;
+        });
+    } else {
+        part.each_two([&](float a, float b) {
+            uint64_t x, y;
+            kept_masses(a, b, x, y);
+            mass += x + y;
+            ties += (a == keep.value) + (b == keep.value);
+        });
+    }
     mass = warp_fold<int64_t, OP_SUM>((int64_t)mass);
     ties = warp_fold<uint32_t, OP_SUM>(ties);
     if (lane == 0) {
@@ -321,94 +800,84 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
     }
     __syncthreads();
     if (warp == 0) {
-        const uint64_t m = (uint64_t)warp_fold<int64_t, OP_SUM>((int64_t)s.warp_mass[lane]);
-        const uint32_t n = warp_fold<uint32_t, OP_SUM>(s.warp_ties[lane]);
+        const uint64_t m = warp_fold<int64_t, OP_SUM>(lane < kSampleWarps ? (int64_t)s.warp_mass[lane] : 0);
+        const uint32_t n = warp_fold<uint32_t, OP_SUM>(lane < kSampleWarps ? s.warp_ties[lane] : 0);
         if (lane == 0) {
-            s.mass = m;
-            s.ties = n;
+            s.block_mass = m;
+            s.block_ties = n;
         }
     }
     cluster.sync();
     auto kept = [&](uint64_t m, uint64_t n) { return m + (n < keep.ties ? n : keep.ties) * tie; };
-    uint64_t all_mass = 0, at_mass = 0;
-    uint32_t all_ties = 0, at_ties = 0;
-    for (uint32_t b = 0; b < blocks; ++b) {
-        const uint64_t m = *cluster.map_shared_rank(&s.mass, b);
-        const uint32_t n = *cluster.map_shared_rank(&s.ties, b);
-        if (b < block) {
-            at_mass += m;
-            at_ties += n;
-        }
-        all_mass += m;
-        all_ties += n;
-    }
+    const uint64_t all = kept((uint64_t)sum_over_blocks((int64_t &)s.block_mass, blocks), sum_over_blocks(s.block_ties, blocks));
+    uint64_t at_mass = (uint64_t)sum_over_blocks((int64_t &)s.block_mass, block);
+    uint32_t at_ties = sum_over_blocks(s.block_ties, block);
     cluster.sync();  // the last reads of other blocks' memory
-    const uint64_t all = kept(all_mass, all_ties);
-    const float u = p.uniform[row];
-    const uint64_t point = ::min((uint64_t)((u > 0.0f ? (double)fminf(u, 1.0f) : 0.0) * (double)all), all - 1);
-    // The warp in whose part the running sum passes the point walks its part.
-    for (uint32_t w = 0; w < warp; ++w) {
-        at_mass += s.warp_mass[w];
-        at_ties += s.warp_ties[w];
-    }
-    if (point < kept(at_mass, at_ties) || point >= kept(at_mass + mass, at_ties + ties)) return;
-    for (uint32_t q0 = part.begin; q0 < part.end; q0 += 32) {
+    const uint64_t point = point_of(all, u);
+    // The block in whose part the running sum passes the point walks through
+    // the part of its warp in which it does, a vector a thread.
+    if (point < kept(at_mass, at_ties)) return;
+    const uint64_t warps_mass = lane < kSampleWarps ? s.warp_mass[lane] : 0, upto_mass = warp_scan(warps_mass);
+    const uint32_t warps_ties = lane < kSampleWarps ? s.warp_ties[lane] : 0, upto_ties = (uint32_t)warp_scan(warps_ties);
+    const uint32_t past = __ballot_sync(kFullMask, point < kept(at_mass + upto_mass, at_ties + upto_ties));
+    if (!past) return;
+    const uint32_t owner = __ffs(past) - 1;
+    at_mass += shfl_idx(upto_mass - warps_mass, owner);
+    at_ties += shfl_idx(upto_ties - warps_ties, owner);
+    const RowPart<T> theirs(part.row, p.vocab, blocks * kSampleWarps, block * kSampleWarps + owner);
+    for (uint32_t q0 = theirs.begin; q0 < theirs.end; q0 += kSampleThreads) {
         constexpr int V = RowPart<T>::V;
-        float v[V];
-        uint64_t m[V], sum = 0;
+        const uint32_t q = q0 + threadIdx.x;
+        const auto v = bitcast<Pack<T, V>>(theirs.load(q));
+        uint64_t m[V], step_mass = 0, more_mass, more_ties;
         uint32_t n = 0;
-        if (q0 + lane < part.end) part.load(q0 + lane, v);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            m[j] = 0;
-            if (q0 + lane >= part.end || !(v[j] == v[j])) v[j] = NAN;
-            else if (ordered_key(v[j]) > keep.key) m[j] = weigh.kept_mass(v[j]);
-            sum += m[j];
-            n += v[j] == v[j] && ordered_key(v[j]) == keep.key;
+        for (int j = 0; j < V; j += 2) {
+            kept_masses(to_f32(v.e[j]), to_f32(v.e[j + 1]), m[j], m[j + 1]);
+            step_mass += m[j] + m[j + 1];
+            n += (to_f32(v.e[j]) == keep.value) + (to_f32(v.e[j + 1]) == keep.value);
         }
-        uint64_t end_mass = at_mass + warp_scan(sum);
-        const uint64_t end_ties = at_ties + warp_scan((uint64_t)n);
-        const bool here = point >= kept(end_mass - sum, end_ties - n) && point < kept(end_mass, end_ties);
-        if (here) {
-            uint64_t run_mass = end_mass - sum;
-            uint64_t run_ties = end_ties - n;
+        uint64_t run_mass = at_mass + block_scan(step_mass, s, more_mass), run_ties = at_ties + block_scan(n, s, more_ties);
+        at_mass += more_mass;
+        at_ties += (uint32_t)more_ties;
+        if (point < kept(run_mass + step_mass, run_ties + n) && point >= kept(run_mass, run_ties)) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                if (!(v[j] == v[j])) continue;
+                const float l = to_f32(v.e[j]);
                 const uint64_t before = kept(run_mass, run_ties);
                 run_mass += m[j];
-                run_ties += ordered_key(v[j]) == keep.key;
+                run_ties += l == keep.value;
                 if (point >= before && point < kept(run_mass, run_ties)) {
-                    p.tokens[row] = (int64_t)(q0 + lane) * V - part.lead + j;
-                    p.probs[row] = (float)(weigh.weight(v[j]) * weigh.unit / (double)all);
+                    p.tokens[row] = (int64_t)q * V - part.lead + j;
+                    p.probs[row] = (float)weigh.share(l, all);
                 }
             }
         }
-        if (__any_sync(kFullMask, here)) return;
-        at_mass = shfl_idx(end_mass, 31);
-        at_ties = (uint32_t)shfl_idx(end_ties, 31);
+        if (point < kept(at_mass, at_ties)) return;
     }
 }
 
 }  // namespace
 
 heph_status launch_sample(const SampleArgs &a, int sm_count, cudaStream_t stream) {
-    // A row's blocks (a cluster) share its passes while there are fewer rows
-    // than SMs and a block still has some work.
+    // A row's blocks (a cluster) share its passes: as many as there are SMs
+    // for all rows, while each still has some work; and, as rows may differ
+    // much in theirs, never over a share of 64 K logits each.  Measured on one
+    // B200 with 1 / 2 / 4 / 8 blocks a row: 1 row of 131072 43 / 30 / 24 / 21
+    // us, 128 of 50257 28.7 / 32 / 46 / 69, 256 of 131072, each with settings
+    // of its own, 280 / 192 / 179 / 228.
     uint32_t blocks = 1;
-    while (blocks < kMaxCluster && (uint64_t)a.rows * blocks * 2 <= (uint32_t)sm_count && a.vocab / (blocks * 2) >= 4096)
+    while (blocks < kMaxCluster && (((uint64_t)a.rows * blocks * 2 <= (uint32_t)sm_count && a.vocab / (blocks * 2) >= 4096) ||
+                                    a.vocab / blocks >= 65536))
         blocks *= 2;
-    // vocab x 2^scale_bits stays below 2^62.
+    // vocab x 2^scale_bits stays below 2^62, and a mass below 2^52.
     const int bits = 32 - __builtin_clz(a.vocab);
     const SampleParams p{a.logits.ptr, a.logits.stride, a.uniform, a.temperature, a.top_p, a.min_p, a.top_k,
-                         a.temperature_all, a.top_p_all, a.min_p_all, a.top_k_all, a.vocab, std::min(52, 62 - bits),
+                         a.temperature_all, a.top_p_all, a.min_p_all, a.top_k_all, a.vocab, std::min(50, 62 - bits),
                          a.tokens, a.probs};
     return dispatch_row_dtype(a.dtype, [&]<typename T>() -> heph_status {
-        HEPH_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           sizeof(SampleShared)),
-                      HEPH_DISPATCH_FAILED, "token sampling shared memory");
-        return launch_clusters("token sampling", sample_kernel<T>, dim3(a.rows * blocks), dim3(kSampleThreads), blocks,
-                               sizeof(SampleShared), stream, p);
+        return launch_clusters("token sampling", sample_kernel<T>, dim3(a.rows * blocks), dim3(kSampleThreads), blocks, 0,
+                               stream, p);
     });
 }
 
