@@ -2,22 +2,27 @@
 
 Every translation unit under ``csrc/`` is compiled to an object in
 ``_build/`` (in parallel, skipping up-to-date objects) and linked into
-``hephaestus_b200/libheph_b200.so``.  Runs without a GPU (nvcc
+``hephaestus_b200/libheph_b200.so``; ``csrc/torch_rows.cpp`` is compiled with
+the host compiler against torch's headers and linked with that library into
+the CPython module ``hephaestus_b200/_torch_rows.so``.  Runs without a GPU (nvcc
 cross-compiles).  ``python hephaestus_b200/build.py [--verbose-ptxas]``.
 """
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libheph_b200.so")
+TORCH_MODULE = os.path.join(PKG, "_torch_rows.so")
 INCLUDE = os.path.join(ROOT, "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -59,6 +64,32 @@ def _compile(src: str, verbose_ptxas: bool) -> str:
     return obj
 
 
+def build_torch_module(force: bool = False) -> str:
+    """``_torch_rows.so``: the torch boundary of the row operators, beside LIB."""
+    src = os.path.join(CSRC, "torch_rows.cpp")
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        raise RuntimeError("torch is needed to build _torch_rows.so")
+    torch_dir = os.path.dirname(spec.origin)
+    newest_dep = max(os.path.getmtime(p) for p in [src, __file__, spec.origin] + headers())
+    if os.path.exists(TORCH_MODULE) and os.path.getmtime(TORCH_MODULE) >= newest_dep and not force:
+        return TORCH_MODULE
+    cuda_home = os.path.dirname(os.path.dirname(nvcc()))
+    lib_dir = os.path.join(torch_dir, "lib")
+    tmp = TORCH_MODULE + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-fPIC", "-shared", "-Wall", "-D_GLIBCXX_USE_CXX11_ABI=1",
+           "-I", INCLUDE, "-isystem", os.path.join(torch_dir, "include"),
+           "-isystem", os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(cuda_home, "include"),
+           src, "-o", tmp, "-L", PKG, "-l:libheph_b200.so", "-L", lib_dir, "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{lib_dir}"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed on {src}:\n{res.stderr}")
+    os.replace(tmp, TORCH_MODULE)
+    return TORCH_MODULE
+
+
 def build(verbose_ptxas: bool = False, force: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     srcs = sources()
@@ -69,6 +100,7 @@ def build(verbose_ptxas: bool = False, force: bool = False) -> str:
         objs = list(ex.map(lambda s: _compile(s, verbose_ptxas), srcs))
     if (os.path.exists(LIB) and not force and
             os.path.getmtime(LIB) >= max(os.path.getmtime(o) for o in objs)):
+        build_torch_module()
         return LIB
     tmp = LIB + ".tmp"
     cmd = [nvcc(), *ARCH, "-shared", "-o", tmp, *objs, "-ldl"]
@@ -76,6 +108,7 @@ def build(verbose_ptxas: bool = False, force: bool = False) -> str:
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stderr}")
     os.replace(tmp, LIB)
+    build_torch_module(force)
     return LIB
 
 

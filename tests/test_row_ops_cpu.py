@@ -34,7 +34,9 @@ def test_norm_refusals():
     refused("power of two", T.rms_norm_fp8, X, group=24)
     refused("power of two", T.rms_norm_fp8, X, group=8)
     refused("dsum must be", T.rms_norm_backward, X, X, dsum=X.half())
-    refused("residual has shape", T.rms_norm_backward, X[:1], X)
+    refused("dy has shape", T.rms_norm_backward, X[:1], X)
+    refused("s must have", T.rms_norm_backward, X.t(), X.t())
+    refused("must be a torch tensor", T.rms_norm, None)
     refused("needs CUDA tensors", T.rms_norm, X, torch.zeros(64))
 
 
