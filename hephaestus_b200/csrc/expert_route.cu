@@ -35,14 +35,14 @@ __device__ __forceinline__ float exp_below(float l, float m) { return l == m ? 1
 // Weight of the row's lane-th choice (logit l, chosen or not).  m, z: maximum
 // and sum of exp(l - m) over the row, of a softmax that is not renormalised.
 __device__ __forceinline__ float choice_weight(float l, bool chosen, bool sigmoid, bool renormalize, float m, float z) {
-    if (!renormalize) return !chosen ? 0.0f : sigmoid ? 1.0f / (1.0f + expf(-l)) : exp_below(l, m) / z;
+    if (!renormalize) return !chosen ? 0.0f : sigmoid ? 1.0f / (1.0f + expf(-l)) : __fdividef(exp_below(l, m), z);
     // Ratios of scores need no row sum, and hold where every score underflows:
     // sigmoid(l) = exp(min(l, 0)) / (1 + exp(-|l|)).
     const float top = key_value(__reduce_max_sync(kFullMask, chosen ? ordered_number(l) : ordered_number(-INFINITY)));
     float s = 0.0f;
-    if (chosen) s = sigmoid ? expf(fminf(l, 0.0f) - fminf(top, 0.0f)) / (1.0f + expf(-fabsf(l))) : exp_below(l, top);
+    if (chosen) s = sigmoid ? __fdividef(expf(fminf(l, 0.0f) - fminf(top, 0.0f)), 1.0f + expf(-fabsf(l))) : exp_below(l, top);
     const float sum = warp_sum(s);
-    return sum > 0.0f ? s / sum : 0.0f;
+    return sum > 0.0f ? __fdividef(s, sum) : 0.0f;
 }
 
 // N adjacent elements of a row from element `e` on; those past `end` are -inf.
@@ -92,100 +92,144 @@ __device__ __forceinline__ float fast_sigmoid(float l) {
     return r;
 }
 
-// The choice in 64 bits, for rows where 32 leave it open: a warp per row, lane
-// i holds experts i N ... i N + N - 1.
-template <typename T, int N> __device__ __noinline__ int32_t choose_exactly(const RouteParams &p, const T *src) {
+// Whether the values of the groups that stay and of those that go (by lane) are
+// further apart than what 32 bits may be off by: `least` for their scores, and
+// roundings of their sums of |c| size_of.
+__device__ __forceinline__ bool groups_apart(float value, float size_of, bool stays, bool is_group, float least) {
+    const uint32_t key = ordered_number(value);
+    const uint32_t low = __reduce_min_sync(kFullMask, stays ? key : ~0u);
+    const uint32_t high = __reduce_max_sync(kFullMask, !stays && is_group ? key : 0u);
+    const float size = __uint_as_float(__reduce_max_sync(kFullMask, is_group ? __float_as_uint(size_of) : 0u));
+    // -inf is exact: a group with nothing to choose.
+    return !high || !(key_value(low) - key_value(high) <= least + 0x1p-22f * size);
+}
+
+// score + bias of the row's experts in 64 bits, lane i's N from i N on; -inf
+// where an expert may not be chosen.  Written out once (unroll 1): few rows
+// come here, and what they wait for is mostly instructions.
+template <typename T, int N>
+__device__ __forceinline__ void exact_values(const RouteParams &p, const T *src, float m, double (&c)[N]) {
     const uint32_t lane = threadIdx.x & 31;
-    float l[N], m = -INFINITY;
-    load_run<T, N>(src, lane * N, p.experts, l);
-    uint32_t open = 0;  // experts that may still be chosen, a bit per j
-    double c[N];
-#pragma unroll
+    double total = 0.0;
+#pragma unroll 1
     for (int j = 0; j < N; ++j) {
-        if (!(l[j] == l[j])) l[j] = -INFINITY;
-        m = fmaxf(m, l[j]);
-        open |= (l[j] > -INFINITY ? 1u : 0u) << j;
-        c[j] = l[j];
+        const uint32_t e = lane * N + j;
+        const float l = e < p.experts ? to_f32(src[e]) : -INFINITY;
+        const double x = exp(p.sigmoid ? -(double)l : l == m ? 0.0 : (double)l - (double)m);
+        c[j] = !(l > -INFINITY) ? -INFINITY : p.sigmoid ? 1.0 / (1.0 + x) : x;
+        if (!p.sigmoid && l > -INFINITY) total += x;
     }
-    m = warp_max(m);
-    if (p.bias || p.groups > 1) {
-        double total = 0.0;
-#pragma unroll
+    if (!p.sigmoid) total = warp_fold<double, OP_SUM>(total);
+#pragma unroll 1
+    for (int j = 0; j < N; ++j) {
+        const uint32_t e = lane * N + j;
+        if (!(c[j] > -INFINITY)) continue;
+        if (!p.sigmoid) c[j] /= total;
+        if (p.bias) c[j] += p.bias[e];
+        if (!(c[j] > -INFINITY)) c[j] = -INFINITY;
+    }
+}
+
+// The groups that stay, a bit each, in 64 bits.
+template <typename T, int N> __device__ __noinline__ uint32_t exact_groups(const RouteParams &p, const T *src, float m) {
+    const uint32_t lane = threadIdx.x & 31;
+    double c[N], mine = -INFINITY;  // of lane g: the value of group g
+    exact_values<T, N>(p, src, m, c);
+#pragma unroll 1
+    for (uint32_t g = 0; g < p.groups; ++g) {
+        const uint32_t begin = g * p.group_size;
+        double a = -INFINITY, b = -INFINITY;  // best and second
+        if (lane * N + N > begin && lane * N < begin + p.group_size) {
+#pragma unroll 1
+            for (int j = 0; j < N; ++j) {
+                if (lane * N + j < begin || lane * N + j >= begin + p.group_size) continue;
+                b = fmax(b, fmin(a, c[j]));
+                a = fmax(a, c[j]);
+            }
+        }
+#pragma unroll 1
+        for (int d = 16; d > 0; d >>= 1) {
+            const double oa = shfl_xor(a, d), ob = shfl_xor(b, d);
+            b = fmax(fmax(b, ob), fmin(a, oa));
+            a = fmax(a, oa);
+        }
+        if (p.top2 && b > -INFINITY) a += b;
+        if (lane == g) mine = a;
+    }
+    uint32_t ahead = 0;
+    for (uint32_t g = 0; g < p.groups; ++g) {
+        const double o = shfl_idx(mine, g);
+        ahead += o > mine || (o == mine && g < lane);
+    }
+    return __ballot_sync(kFullMask, lane < p.groups && ahead < p.groups_kept);
+}
+
+// Lane i's choice in 64 bits, for rows of more near candidates than lanes;
+// `kept`: the groups that stay.
+template <typename T, int N> __device__ __noinline__ int32_t exact_choice(const RouteParams &p, const T *src, float m, uint32_t kept) {
+    const uint32_t lane = threadIdx.x & 31;
+    double c[N];
+    if (p.bias) {
+        exact_values<T, N>(p, src, m, c);
+    } else {
         for (int j = 0; j < N; ++j) {
-            const double d = l[j];
-            if (p.sigmoid) c[j] = 1.0 / (1.0 + exp(-d));
-            else c[j] = !(open >> j & 1u) ? 0.0 : l[j] == m ? 1.0 : exp(d - m);
-            total += c[j];
-        }
-        if (!p.sigmoid) {
-            total = warp_fold<double, OP_SUM>(total);
-#pragma unroll
-            for (int j = 0; j < N; ++j) c[j] /= total;
-        }
-        if (p.bias) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const uint32_t e = lane * N + j;
-                if (e < p.experts) c[j] += p.bias[e];
-                if (!(c[j] > -INFINITY)) open &= ~(1u << j);
-            }
-        }
-        if (p.groups > 1) {
-            const uint32_t size = p.group_size;
-            double mine = -INFINITY;  // lane g: the value of group g
-            for (uint32_t g = 0; g < p.groups; ++g) {
-                double a = -INFINITY, b = -INFINITY;  // best and second
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const uint32_t e = lane * N + j;
-                    if ((open >> j & 1u) && e >= g * size && e - g * size < size) {
-                        b = fmax(b, fmin(a, c[j]));
-                        a = fmax(a, c[j]);
-                    }
-                }
-#pragma unroll
-                for (int d = 16; d > 0; d >>= 1) {
-                    const double oa = shfl_xor(a, d), ob = shfl_xor(b, d);
-                    b = fmax(fmax(b, ob), fmin(a, oa));
-                    a = fmax(a, oa);
-                }
-                if (p.top2 && b > -INFINITY) a += b;
-                if (lane == g) mine = a;
-            }
-            uint32_t ahead = 0;
-            for (uint32_t g = 0; g < p.groups; ++g) {
-                const double o = shfl_idx(mine, g);
-                ahead += o > mine || (o == mine && g < lane);
-            }
-            const uint32_t kept = __ballot_sync(kFullMask, lane < p.groups && ahead < p.groups_kept);
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const uint32_t e = lane * N + j;
-                if (e < p.experts && !(kept >> (e / size) & 1u)) open &= ~(1u << j);
-            }
-            if (!p.bias) {
-#pragma unroll
-                for (int j = 0; j < N; ++j) c[j] = l[j];
-            }
+            const float l = lane * N + j < p.experts ? to_f32(src[lane * N + j]) : -INFINITY;
+            c[j] = l == l ? l : -INFINITY;
         }
     }
+    for (int j = 0; j < N; ++j)
+        if (p.groups > 1 && lane * N + j < p.experts && !(kept >> ((lane * N + j) / p.group_size) & 1u)) c[j] = -INFINITY;
     int32_t pick = -1;
+#pragma unroll 1
     for (uint32_t i = 0; i < p.k; ++i) {
         double best = -INFINITY;
         uint32_t at = 0xffffffffu;
-#pragma unroll
+#pragma unroll 1
         for (int j = 0; j < N; ++j) {
-            if ((open >> j & 1u) && (at == 0xffffffffu || c[j] > best)) {
+            if (c[j] > best) {
                 best = c[j];
                 at = lane * N + j;
             }
         }
         warp_arg_fold<double, OP_MAX>(best, at);
         if (at == 0xffffffffu) break;  // nothing left, for every lane
-        if (at / N == lane) open &= ~(1u << (at % N));
+        if (at / N == lane) c[at % N] = -INFINITY;
         if (lane == i) pick = (int32_t)at;
     }
     return pick;
+}
+
+// The rank of candidate `mine` (of the first `count` lanes, one each) by the
+// 64-bit values of score + bias or of the logits, equal ones by expert.
+template <typename T, int N>
+__device__ __noinline__ void exact_rank(const RouteParams &p, const T *src, uint32_t mine, uint32_t lane, uint32_t count, float m,
+                                        double *values, const uint2 *candidates, uint32_t &rank) {
+    const uint32_t lanes = (uint32_t)((1ull << count) - 1);
+    const float l = to_f32(src[mine]);
+    double c = l;
+    if (p.bias) {
+        if (p.sigmoid) {
+            c = 1.0 / (1.0 + exp(-c));
+        } else {
+            double z = 0.0;  // of the row, the experts dealt to the lanes
+            for (uint32_t e = lane; e < p.experts; e += count) {
+                const float o = to_f32(src[e]);
+                z += o == m ? 1.0 : o > -INFINITY ? exp((double)o - (double)m) : 0.0;
+            }
+            values[lane] = z;
+            __syncwarp(lanes);
+            z = 0.0;
+            for (uint32_t i = 0; i < count; ++i) z += values[i];
+            __syncwarp(lanes);
+            c = (l == m ? 1.0 : exp(c - (double)m)) / z;
+        }
+        c += p.bias[mine];
+    }
+    values[lane] = c;
+    __syncwarp(lanes);
+    rank = 0;
+    for (uint32_t i = 0; i < count; ++i) rank += values[i] > c || (values[i] == c && candidates[i].y < mine);
+    __syncwarp(lanes);
 }
 
 // Sorts N values a lane into falling order (Batcher's odd-even merges).
@@ -207,8 +251,9 @@ template <int N> __device__ __forceinline__ void sort_falling(uint32_t (&v)[N]) 
 
 // A warp per row, lane i holds experts i N ... i N + N - 1.  The choice is
 // made in 32 bits and checked: where a gap that decides something is not
-// wider than what 32 bits may be off by, the row is chosen again in 64 bits
-// (about 1 row in 100 with a sigmoid and a bias).
+// wider than what 32 bits may be off by, 64 bits decide: of the candidates
+// (about 2 rows in 1000 with a sigmoid and a bias), or, where the groups are
+// in doubt (1 in 30000), of the whole row.
 template <typename T, int N> __global__ void __launch_bounds__(32 * kRouteWarps, N <= 8 ? 10 : 1)
 route_kernel(const __grid_constant__ RouteParams p) {
     constexpr uint32_t kLow = N - 1;  // the low bits of a key hold N - 1 - j
@@ -228,10 +273,11 @@ route_kernel(const __grid_constant__ RouteParams p) {
             z += !(c[j] > -INFINITY) ? 0.0f : c[j] == m ? 1.0f : p.renormalize ? fast_exp(c[j] - m) : expf(c[j] - m);
         z = warp_sum(z);
     }
-    // A score is off by less than 2^-18 (two units of the fast exp, its
-    // rounded exponent x with x e^-x, ten levels of the sum, whose terms'
-    // exponents average below ln 1024, and the quotient).
-    constexpr float kScoreOff = 0x1p-18f;
+    // What a score may be off by.  Sigmoid: a quarter of the exp's error (a
+    // unit and a half, and its rounded exponent l with |l| s (1 - s) < 1/4),
+    // half a unit of the sum and a unit of the reciprocal, below 2^-22.  Softmax: those, ten levels of the sum, whose
+    // terms' exponents average below ln 1024, and the quotient, below 2^-18.
+    const float score_off = p.sigmoid ? 0x1p-22f : 0x1p-18f;
     const float inverse = 1.0f / z;
     auto score = [&](float l) { return p.sigmoid ? fast_sigmoid(l) : l == m ? inverse : fast_exp(l - m) * inverse; };
     // A key in the order of the choice: of score + bias, or of the logit; 0
@@ -252,9 +298,9 @@ route_kernel(const __grid_constant__ RouteParams p) {
     }
     // Half of what two keys' values may differ by and yet be in the other
     // order: the score's error, a rounding of the sum, a unit of the last kept bit.
-    const float key_off = p.bias ? kScoreOff : 0.0f;
+    const float key_off = p.bias ? score_off : 0.0f;
     constexpr float kKeyStep = 0x1p-23f * (N + 1);
-    bool sure = true;
+    uint32_t kept = 0;  // the groups that stay, a bit each
     if (p.groups > 1 && !p.group_lanes) {
         // Groups of any size: each group's best two of all lanes, in turn.
         float mine = -INFINITY, size_of = 0.0f;  // lane g: the value of group g
@@ -283,25 +329,38 @@ route_kernel(const __grid_constant__ RouteParams p) {
         }
         uint32_t ahead = 0;
         for (uint32_t g = 0; g < p.groups; ++g) {
-            const float o = shfl_idx(mine, g), size = shfl_idx(size_of, g);
+            const float o = shfl_idx(mine, g);
             ahead += o > mine || (o == mine && g < lane);
-            if (lane < p.groups && g != lane && fabsf(o - mine) <= 4.0f * kScoreOff + kKeyStep * (size + size_of)) sure = false;
         }
-        const uint32_t kept = __ballot_sync(kFullMask, lane < p.groups && ahead < p.groups_kept);
+        const bool stays = lane < p.groups && ahead < p.groups_kept;
+        kept = groups_apart(mine, size_of, stays, lane < p.groups, 4.0f * score_off)
+                   ? __ballot_sync(kFullMask, stays)
+                   : exact_groups<T, N>(p, src, m);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const uint32_t e = lane * N + j;
             if (e < p.experts && !(kept >> (e / p.group_size) & 1u)) key[j] = 0;
         }
     }
+    // Best and second of the lane's experts, to value its group by.
+    float best = -INFINITY, second = -INFINITY;
+    if (p.group_lanes && p.bias) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            second = fmaxf(second, fminf(best, c[j]));
+            best = fmaxf(best, c[j]);
+        }
+    }
     sort_falling<N>(key);  // each lane's; the row's next is the largest head
     if (p.groups > 1 && p.group_lanes) {
         // A group is a power of two of whole lanes, which share the comparisons.
-        auto value = [&](uint32_t k) {
-            const float v = key_value(k & ~kLow);
-            return !k ? -INFINITY : p.bias ? v : score(v);
-        };
-        float a = value(key[0]), b = N > 1 ? value(key[N > 1]) : -INFINITY;  // best and second
+        float a = best, b = second;
+        if (!p.bias) {
+            // Without a bias the order is that of the logits: two scores will do.
+            auto value = [&](uint32_t k) { return k ? score(to_f32(src[lane * N + kLow - (k & kLow)])) : -INFINITY; };
+            a = value(key[0]);
+            b = N > 1 ? value(key[N > 1]) : -INFINITY;
+        }
         for (uint32_t d = 1; d < p.group_lanes; d *= 2) {
             const float oa = shfl_xor(a, d), ob = shfl_xor(b, d);
             b = fmaxf(fmaxf(b, ob), fminf(a, oa));
@@ -309,54 +368,111 @@ route_kernel(const __grid_constant__ RouteParams p) {
         }
         if (!p.top2 || !(b > -INFINITY)) b = 0.0f;
         const float mine = a + b, size_of = mine > -INFINITY ? fabsf(a) + fabsf(b) : 0.0f;
-        // A logit's unit, |l| kKeyStep, is one of its score times |l| at most:
-        // |x s'(x)| < 1 for a sigmoid, and |l| <= |max| + (max - l) for a softmax.
-        const float step = p.bias ? kKeyStep : kKeyStep * (1.0f + fabsf(m)), least = 4.0f * (kScoreOff + kKeyStep);
         const uint32_t own = lane >> p.group_shift, share = lane & (p.group_lanes - 1);
         uint32_t ahead = 0;
         for (uint32_t g = share; g < p.groups + share; g += p.group_lanes) {
             const uint32_t from = g << p.group_shift;
-            const float o = __shfl_sync(kFullMask, mine, from), size = __shfl_sync(kFullMask, size_of, from);
-            if (g < p.groups && own < p.groups && g != own) {
-                ahead += o > mine || (o == mine && g < own);
-                if (fabsf(o - mine) <= least + step * (size + size_of)) sure = false;
-            }
+            const float o = __shfl_sync(kFullMask, mine, from);
+            if (g < p.groups) ahead += o > mine || (o == mine && g < own);
         }
         for (uint32_t d = 1; d < p.group_lanes; d *= 2) ahead += __shfl_xor_sync(kFullMask, ahead, d);
-        if (ahead >= p.groups_kept) {
+        bool stays = own < p.groups && ahead < p.groups_kept;
+        if (groups_apart(mine, size_of, stays, own < p.groups, 4.0f * score_off)) {
+            kept = __reduce_or_sync(kFullMask, stays ? 1u << own : 0u);
+        } else {
+            kept = exact_groups<T, N>(p, src, m);
+            stays = own < p.groups && (kept >> own & 1u);
+        }
+        if (!stays) {
 #pragma unroll
             for (int j = 0; j < N; ++j) key[j] = 0;
         }
     }
-    __shared__ uint2 winners[kRouteWarps][32];
-    uint2 *won_by = winners[threadIdx.x >> 5];
+    // The row's first k, and one more to check the last by: of lane i the
+    // i-th key, its low bits cleared, and its expert.  Key 0: none is left.
+    __shared__ uint2 listed[kRouteWarps][32], winners[kRouteWarps][32];
+    __shared__ double values[kRouteWarps][32];
+    uint2 *candidates = listed[threadIdx.x >> 5], *won_by = winners[threadIdx.x >> 5];
     const uint32_t turns = min(p.k + 1, 32u), lower = (1u << lane) - 1;
     won_by[lane] = make_uint2(0, 0);
-    __syncwarp();
-    for (uint32_t i = 0; i < turns; ++i) {
-        const uint32_t head = key[0] & ~kLow;
-        const uint32_t best = __reduce_max_sync(kFullMask, head);
-        const uint32_t owners = __ballot_sync(kFullMask, head == best);
-        if (head == best && !(owners & lower)) {  // the lowest of them
-            won_by[i] = make_uint2(key[0], lane * N);
+    auto entry = [&](uint32_t k) { return make_uint2(k & ~kLow, lane * N + kLow - (k & kLow)); };
+    // k + 1 lanes have a key at or above the (k+1)-th largest head: the
+    // candidates are the keys that reach it, few more than k + 1.
+    // (And the keys that are less than the margin below it, which 64 bits may
+    // place before it.)
+    auto margin = [&](float v) { return 2.0f * (key_off + fabsf(v) * kKeyStep) + 0x1p-120f; };
+    // Keys of 16-bit logits themselves lose nothing in the low bits: equal
+    // keys are equal logits, which the index settles.
+    const bool exact = !p.bias && sizeof(T) == 2;
+    uint32_t least = 1, count = 0;
+    if (turns <= 13) {
+        uint32_t head = key[0] & ~kLow;
+        for (uint32_t i = 0; i < turns; ++i) {
+            least = __reduce_max_sync(kFullMask, head);
+            if (head == least) head = 0;
+        }
+        if (least && !exact) least = ordered_number(key_value(least) - 2.0f * margin(key_value(least))) & ~kLow;
+        least = max(least, 1u);
 #pragma unroll
-            for (int j = 0; j + 1 < N; ++j) key[j] = key[j + 1];
-            key[N - 1] = 0;
+        for (int j = 0; j < N; ++j) {
+            const uint32_t reach = __ballot_sync(kFullMask, (key[j] & ~kLow) >= least);
+            if (!reach) break;
+            const uint32_t at = count + __popc(reach & lower);
+            if ((reach >> lane & 1u) && at < 32) candidates[at] = entry(key[j]);
+            count += __popc(reach);
+        }
+    } else {
+        count = 33;
+    }
+    __syncwarp();
+    if (count <= 32) {
+        // Each lane ranks one of them; equal keys by expert.
+        const uint2 mine = lane < count ? candidates[lane] : make_uint2(0, 0);
+        uint32_t rank = 0;
+        for (uint32_t i = 0; i < count; ++i) {
+            const uint2 o = candidates[i];
+            rank += o.x > mine.x || (o.x == mine.x && o.y < mine.y);
+        }
+        if (lane < count) won_by[rank] = mine;
+        __syncwarp();
+        if (!exact) {
+            const uint32_t next = lane < 31 ? won_by[lane + 1].x : 0;
+            const float a = key_value(won_by[lane].x);
+            const bool near = lane < p.k && next && a - key_value(next) <= margin(a);
+            if (__any_sync(kFullMask, near)) {
+                // Ranks by the 64-bit values of the candidates.
+                __syncwarp();
+                if (lane < count) {
+                    exact_rank<T, N>(p, src, mine.y, lane, count, m, values[threadIdx.x >> 5], candidates, rank);
+                    won_by[rank] = mine;
+                }
+            }
+        }
+    } else {
+        // Many to choose, or few lanes to choose from: one after the other.
+        for (uint32_t i = 0; i < turns; ++i) {
+            const uint32_t head = key[0] & ~kLow;
+            const uint32_t best = __reduce_max_sync(kFullMask, head);
+            const uint32_t owners = __ballot_sync(kFullMask, head == best);
+            if (best && head == best && !(owners & lower)) {  // the lowest of them
+                won_by[i] = entry(key[0]);
+#pragma unroll
+                for (int j = 0; j + 1 < N; ++j) key[j] = key[j + 1];
+                key[N - 1] = 0;
+            }
         }
     }
     __syncwarp();
-    const uint2 won = won_by[lane];  // key 0: none is left
-    // Equal keys of the logits themselves (16-bit types lose nothing in the
-    // low bits) are equal logits, which the lanes' order has settled.
-    const bool exact = !p.bias && sizeof(T) == 2;
-    if (!exact && lane < p.k && won.x) {
+    const uint2 won = won_by[lane];
+    bool sure = true;
+    if (count > 32 && !exact && lane < p.k && won.x) {
         const uint32_t next = lane < 31 ? won_by[lane + 1].x : 0;
-        const float a = key_value(won.x & ~kLow), b = key_value(next & ~kLow);
-        if (next && a - b <= 2.0f * (key_off + fabsf(a) * kKeyStep) + 0x1p-120f) sure = false;
+        const float a = key_value(won.x);
+        if (next && a - key_value(next) <= margin(a)) sure = false;
+        if (p.k == 32) sure = false;  // there is no lane for the 33rd
     }
-    int32_t pick = won.x && lane < p.k ? (int32_t)(won.y + kLow - (won.x & kLow)) : -1;
-    if (p.k == 32 && !exact) sure = false;  // there is no lane for the 33rd
-    if (!__all_sync(kFullMask, sure)) pick = choose_exactly<T, N>(p, src);
+    int32_t pick = won.x && lane < p.k ? (int32_t)won.y : -1;
+    if (!__all_sync(kFullMask, sure)) pick = exact_choice<T, N>(p, src, m, kept);
     const float logit = pick >= 0 ? to_f32(src[pick]) : 0.0f;
     const float w = choice_weight(logit, pick >= 0, p.sigmoid, p.renormalize, m, z);
     if (lane < p.k) {
@@ -380,27 +496,20 @@ struct RouteGradParams {
 // else d(log s_j) = scale s_j g_j;  then for a sigmoid dl_j = d(log s_j)
 // (1 - s_j), for a softmax dl_i = d(log s_i) - s_i sum of all d(log s), whose
 // last term vanishes when renormalised.
-template <typename T, int N> __global__ void __launch_bounds__(32 * kRouteWarps) route_grad_kernel(const __grid_constant__ RouteGradParams p) {
+template <typename T, int N> __global__ void __launch_bounds__(32 * kRouteWarps)
+route_grad_kernel(const __grid_constant__ RouteGradParams p) {
+    // The row's gradient of the log scores, by expert; first used to see
+    // whether an expert is named twice.
+    __shared__ __align__(16) float by_expert[kRouteWarps][32 * N];
     const uint32_t lane = threadIdx.x & 31, row = blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
     if (row >= p.rows) return;
     const T *src = static_cast<const T *>(p.logits) + row * p.stride;
-    const bool whole = !p.sigmoid && !p.renormalize;  // every logit has a gradient
-    float l[N], m = -INFINITY, z = 0.0f;
-    if (whole) {
-        load_run<T, N>(src, lane * N, p.experts, l);
+    float *at = by_expert[threadIdx.x >> 5];
+    using Run = Pack<float, N < 4 ? N : 4>;
+    Run *own = reinterpret_cast<Run *>(at + lane * N);
+    constexpr int kRuns = N < 4 ? 1 : N / 4;
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            if (!(l[j] == l[j])) l[j] = -INFINITY;
-            m = fmaxf(m, l[j]);
-        }
-        m = warp_max(m);
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            l[j] = l[j] > -INFINITY ? exp_below(l[j], m) : 0.0f;
-            z += l[j];
-        }
-        z = warp_sum(z);
-    }
+    for (int i = 0; i < kRuns; ++i) own[i] = Run{};
     uint32_t pick = ~0u;
     float logit = 0.0f, g = 0.0f;
     if (lane < p.k) {
@@ -410,22 +519,52 @@ template <typename T, int N> __global__ void __launch_bounds__(32 * kRouteWarps)
             logit = to_f32(src[pick]);
         }
     }
+    const bool whole = !p.sigmoid && !p.renormalize;  // every logit has a gradient
+    float l[N], m = -INFINITY, z = 0.0f;
+    if (whole) {
+        load_run<T, N>(src, lane * N, p.experts, l);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (!(l[j] == l[j])) l[j] = -INFINITY;
+            m = fmaxf(m, l[j]);
+        }
+        m = key_value(__reduce_max_sync(kFullMask, ordered_number(m)));
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            l[j] = l[j] == m ? 1.0f : fast_exp(l[j] - m);
+            z += l[j];
+        }
+        z = m > -INFINITY ? warp_sum(z) : 0.0f;
+    }
     const bool chosen = pick < p.experts && logit > -INFINITY;
     if (!chosen) g = 0.0f;
     const float r = choice_weight(logit, chosen, p.sigmoid, p.renormalize, m, z);
     const float dot = warp_sum(g * r);
     float d = p.scale * r * (p.renormalize ? g - dot : g);
     if (p.sigmoid) d /= 1.0f + expf(logit);
+    __syncwarp();
+    if (chosen) at[pick] = __uint_as_float(lane);
+    __syncwarp();
+    const bool alone = !chosen || at[pick] == __uint_as_float(lane);
+    __syncwarp();
+    if (__all_sync(kFullMask, alone)) {
+        if (chosen) at[pick] = d;
+    } else {
+        // In turn, so that the sum of an expert's does not depend on an order.
+        if (chosen) at[pick] = 0.0f;
+        for (uint32_t i = 0; i < p.k; ++i) {
+            __syncwarp();
+            if (lane == i && chosen) at[pick] += d;
+        }
+    }
+    __syncwarp();
     float dl[N];
+    const float rest = whole && z > 0.0f ? -p.scale * dot / z : 0.0f;
 #pragma unroll
-    for (int j = 0; j < N; ++j) dl[j] = whole && z > 0.0f ? -p.scale * dot * (l[j] / z) : 0.0f;
-    // Choices in turn, so that an expert named twice gets both in order.
-    for (uint32_t i = 0; i < p.k; ++i) {
-        const uint32_t e = __shfl_sync(kFullMask, pick, i);
-        const float add = __shfl_sync(kFullMask, d, i);
+    for (int i = 0; i < kRuns; ++i) {
+        const Run u = own[i];
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (e == lane * N + j) dl[j] += add;
+        for (int j = 0; j < N / kRuns; ++j) dl[i * (N / kRuns) + j] = u.e[j] + (whole ? rest * l[i * (N / kRuns) + j] : 0.0f);
     }
     store_run<T, N>(static_cast<T *>(p.dlogits) + (int64_t)row * p.experts, lane * N, p.experts, dl);
 }
