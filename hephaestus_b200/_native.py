@@ -128,7 +128,8 @@ SIGNATURES = [
                                      _u64, _vp]),
     ("heph_route_experts", _st, [_i, _i, _vp, _i64, _vp, _u64, _u32, _u32, _i, _u32, _u32, _u32, _i, _f32, _vp, _vp, _vp]),
     ("heph_route_experts_backward", _st, [_i, _i, _vp, _i64, _vp, _i64, _vp, _i64, _u64, _u32, _u32, _i, _i, _f32, _vp, _vp]),
-    ("heph_expert_order", _st, [_i, _vp, _u64, _u32, _vp, _vp, _vp, _vp]),
+    ("heph_expert_order_workspace", _st, [_u64, _u32, ctypes.POINTER(_u64)]),
+    ("heph_expert_order", _st, [_i, _vp, _u64, _u32, _vp, _vp, _vp, _vp, _u64, _vp]),
     ("heph_sample_tokens", _st, [_i, _i, _vp, _i64, _u64, _u32, _vp, _vp, _f64, _vp, _i32, _vp, _f64, _vp, _f64, _vp, _vp,
                                  _vp]),
     ("heph_synth_fill", _st, [_vp, _vp, _u64, _u64, _i, _u64, _u64, _vp]),

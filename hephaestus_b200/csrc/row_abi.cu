@@ -279,8 +279,18 @@ extern "C" heph_status heph_route_experts_backward(int ordinal, heph_row_dtype d
     });
 }
 
+extern "C" heph_status heph_expert_order_workspace(uint64_t count, uint32_t experts, uint64_t *out_bytes) {
+    return guarded([&]() -> heph_status {
+        if (!out_bytes) return refuse("null output");
+        if (count > kMaxRows || experts > kMaxExperts) return refuse("expert_order pairs or experts out of range");
+        *out_bytes = expert_order_workspace((uint32_t)count, experts);
+        return HEPH_OK;
+    });
+}
+
 extern "C" heph_status heph_expert_order(int ordinal, const int32_t *picks, uint64_t count, uint32_t experts,
-                                         int32_t *offsets, int32_t *order, int32_t *slot, heph_stream stream) {
+                                         int32_t *offsets, int32_t *order, int32_t *slot, void *workspace,
+                                         uint64_t workspace_bytes, heph_stream stream) {
     return guarded([&]() -> heph_status {
         if (experts < 1 || experts > kMaxExperts)
             return refuse("expert_order takes 1 to " + std::to_string(kMaxExperts) + " experts");
@@ -290,10 +300,16 @@ extern "C" heph_status heph_expert_order(int ordinal, const int32_t *picks, uint
         HEPH_TRY(check_matrix("order", order, 1, count, 0, 4));
         HEPH_TRY(check_matrix("slot", slot, 1, count, 0, 4));
         HEPH_TRY(check_apart("expert_order", {Span(picks, count, 4)},
-                             {Span(offsets, experts + 1, 4), Span(order, count, 4), Span(slot, count, 4)}));
+                             {Span(offsets, experts + 1, 4), Span(order, count, 4), Span(slot, count, 4),
+                              Span(workspace, workspace_bytes, 1)}));
+        const uint64_t need = expert_order_workspace((uint32_t)count, experts);
+        if (need && (!workspace || workspace_bytes < need))
+            return refuse("expert_order needs a workspace of " + std::to_string(need) + " bytes");
+        if (reinterpret_cast<uintptr_t>(workspace) % 16) return refuse("expert_order workspace is not aligned to 16 bytes");
         OnDevice on;
         HEPH_TRY(on.enter(ordinal));
-        return launch_expert_order(picks, (uint32_t)count, experts, offsets, order, slot, static_cast<cudaStream_t>(stream));
+        return launch_expert_order(picks, (uint32_t)count, experts, offsets, order, slot, static_cast<uint32_t *>(workspace),
+                                   static_cast<cudaStream_t>(stream));
     });
 }
 

@@ -11,7 +11,7 @@
 
 namespace heph {
 
-constexpr uint32_t kMaxExperts = 1024;  // a thread each in expert_order
+constexpr uint32_t kMaxExperts = 1024;  // 32 a lane in expert_route
 constexpr uint32_t kMaxChoices = 32;    // a lane each in expert_route
 constexpr uint32_t kMaxGroups = 32;
 
@@ -71,8 +71,9 @@ struct RouteGradArgs {
 };
 heph_status launch_route_backward(const RouteGradArgs &a, cudaStream_t stream);
 
+size_t expert_order_workspace(uint32_t count, uint32_t experts);
 heph_status launch_expert_order(const int32_t *picks, uint32_t count, uint32_t experts, int32_t *offsets,
-                                int32_t *order, int32_t *slot, cudaStream_t stream);
+                                int32_t *order, int32_t *slot, uint32_t *workspace, cudaStream_t stream);
 
 struct SampleArgs {
     heph_row_dtype dtype;

@@ -346,10 +346,13 @@ PyObject *expert_order(PyObject *const *args) {
     const int device = device_of({&experts});
     const int64_t count = experts.numel();
     at::Tensor offsets = empty({num + 1}, at::kInt, device), order = empty({count}, at::kInt, device);
-    at::Tensor slot = empty(experts.sizes(), at::kInt, device);
+    at::Tensor slot = empty(experts.sizes(), at::kInt, device), work;
+    uint64_t bytes = 0;
+    check(heph_expert_order_workspace((uint64_t)count, (uint32_t)num, &bytes));
+    if (bytes) work = empty({(int64_t)bytes}, at::kByte, device);
     check(heph_expert_order(device, (const int32_t *)experts.const_data_ptr(), (uint64_t)count, (uint32_t)num,
                             (int32_t *)offsets.data_ptr(), (int32_t *)order.data_ptr(), (int32_t *)slot.data_ptr(),
-                            stream_of(device)));
+                            bytes ? work.data_ptr() : nullptr, bytes, stream_of(device)));
     return tuple({&offsets, &order, &slot});
 }
 

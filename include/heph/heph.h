@@ -549,9 +549,13 @@ heph_status heph_route_experts_backward(int ordinal, heph_row_dtype dtype, const
  * exclusive scan of the experts' counts), order [count] (the pairs' places,
  * by expert and then by place; -1 past the last), slot [count] (the inverse:
  * where a pair stands in `order`, -1 where its pick is outside [0, experts)).
- * experts <= 1024. */
+ * experts <= 1024.  The workspace (16-byte aligned, of the size the first
+ * call tells; NULL for a size of 0, as up to 65536 pairs) is free again when
+ * the call's work has run. */
+heph_status heph_expert_order_workspace(uint64_t count, uint32_t experts, uint64_t *out_bytes);
 heph_status heph_expert_order(int ordinal, const int32_t *picks, uint64_t count, uint32_t experts,
-                              int32_t *offsets, int32_t *order, int32_t *slot, heph_stream stream);
+                              int32_t *offsets, int32_t *order, int32_t *slot, void *workspace,
+                              uint64_t workspace_bytes, heph_stream stream);
 
 /* Draws a token from every row of `logits`: w_i = exp((l_i - max l) / T).  In
  * the order of falling l (lowest index first among equals) top_k keeps the

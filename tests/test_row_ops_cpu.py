@@ -151,11 +151,15 @@ def test_c_route_refusals():
 
 
 def test_c_order_refusals():
-    good = [0, A, 100, 8, B, C, D, None]
+    good = [0, A, 100, 8, B, C, D, None, 0, None]
     for at, value, message in ((3, 0, "1 to 1024"), (3, 1025, "1 to 1024"), (2, 1 << 31, "out of range"), (1, None, "picks is null"),
                                (4, None, "offsets is null"), (5, None, "order is null"), (6, None, "slot is null"),
-                               (5, A, "alias its inputs"), (6, C + 4, "alias one another"), (4, B + 2, "not aligned")):
+                               (5, A, "alias its inputs"), (6, C + 4, "alias one another"), (4, B + 2, "not aligned"), (2, 200000, "needs a workspace of 3136 bytes")):
         c_refused(message, "heph_expert_order", *(good[:at] + [value] + good[at + 1:]))
+    c_refused("not aligned to 16", "heph_expert_order", *(good[:7] + [0x5000008, 64, None]))
+    need = ctypes.c_uint64()
+    c_refused("null output", "heph_expert_order_workspace", 4, 4, None)
+    c_refused("out of range", "heph_expert_order_workspace", 1 << 31, 4, ctypes.byref(need))
 
 
 def test_c_sample_refusals():

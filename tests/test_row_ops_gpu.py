@@ -301,7 +301,8 @@ def test_route_backward_against_differences(T):
 
 
 @pytest.mark.parametrize("shape,experts", [((1, 1), 1), ((3, 2), 4), ((64, 8), 256), ((31, 1), 7), ((1000, 3), 1024),
-                                           ((4096, 1), 60), ((1025, 4), 33), ((5000, 6), 128), ((40000, 2), 513)])
+                                           ((4096, 1), 60), ((1025, 4), 33), ((5000, 6), 128), ((40000, 2), 513),
+                                           ((65536, 1), 256), ((65537, 1), 1000), ((60000, 5), 31), ((1100000, 2), 64)])
 def test_expert_order(T, shape, experts):
     g = torch.Generator(device="cuda").manual_seed(experts)
     picks = torch.randint(-1, experts, shape, device="cuda", dtype=torch.int32, generator=g)
@@ -550,7 +551,7 @@ def test_leaves_its_surroundings_alone(T):
     picks = torch.randint(0, 9, (777,), device="cuda", dtype=torch.int32)
     pad = torch.full((3, 1000), 5, dtype=torch.int32, device="cuda")
     assert N.lib.heph_expert_order(0, picks.data_ptr(), 777, 9, pad[0, 10:].data_ptr(), pad[1, 10:].data_ptr(),
-                                   pad[2, 10:].data_ptr(), None) == N.OK
+                                   pad[2, 10:].data_ptr(), None, 0, None) == N.OK
     assert bool((pad[:, :10] == 5).all()) and bool((pad[0, 20:] == 5).all()) and bool((pad[1:, 787:] == 5).all())
     assert torch.cuda.current_device() == 0
 
