@@ -83,7 +83,7 @@ struct SampleShared {
     uint32_t listed[2];  // entries in `list`, and in `mass` where that is the second list
     Threshold keep;
     uint32_t found_bin;
-    uint64_t found_above, found_in, kept_mass;
+    uint64_t found_above, found_in;
 };
 
 // Adds a 64-bit mass by two 32-bit atomics, whose order changes nothing.
@@ -144,14 +144,16 @@ template <typename T> struct RowPart {
     }
     // Vector q; what is outside the part or the row is NaN.
     __device__ __forceinline__ uint4 load(uint32_t q) const {
-        return q - whole_begin < whole ? vectors[q] : load_edge(q);
+        if (q - whole_begin < whole) return vectors[q];
+        if (q < end) return load_edge(q);
+        return make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);  // a NaN in every type
     }
     __device__ __noinline__ uint4 load_edge(uint32_t q) const {
         Pack<T, V> u;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const uint32_t at = q * V + j - lead;  // wraps before the row
-            u.e[j] = q < end && at < vocab ? row[at] : from_f32<T>(NAN);
+            u.e[j] = at < vocab ? row[at] : from_f32<T>(NAN);
         }
         return bitcast<uint4>(u);
     }
@@ -577,7 +579,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     const uint32_t row = blockIdx.x / blocks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const RowPart<T> part(static_cast<const T *>(p.logits) + row * p.stride, p.vocab, blocks * kSampleWarps,
                           block * kSampleWarps + warp);
-    const double t = p.temperature ? p.temperature[row] : p.temperature_all;
+    double t = p.temperature ? p.temperature[row] : p.temperature_all;
     const int32_t k = p.top_k ? p.top_k[row] : p.top_k_all;
     const double top_p = p.top_p ? p.top_p[row] : p.top_p_all;
     const double min_p = p.min_p ? p.min_p[row] : p.min_p_all;
@@ -653,6 +655,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         return;
     }
 
+    t = fmax(t, 0x1p-100);  // 1 / t stays a number in 32 bits
     const Weigher weigh(max, t, p.scale_bits, s.roots);
     const double least_w = min_p > 0.0 ? fmin(min_p, 1.0) : 0.0;
     const uint64_t least = (uint64_t)ceil(least_w * (double)(1ull << p.scale_bits));
