@@ -13,7 +13,7 @@ namespace {
 constexpr uint64_t kMaxRows = 0x7fffffff;   // blocks of a grid, 32-bit row numbers
 constexpr uint64_t kMaxCols = 1u << 24;
 constexpr uint64_t kMaxScales = 8192;       // group maxima of a row in 32 KiB of shared memory
-constexpr uint64_t kMaxVocab = 1u << 26;    // masses of 36 bits or more
+constexpr uint64_t kMaxVocab = (1u << 22) - (1u << 16);  // sums of the limbs of masses in 32 bits (sample.cu)
 
 size_t row_dtype_size(heph_row_dtype dt) {
     switch (dt) {

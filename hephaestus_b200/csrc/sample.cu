@@ -53,13 +53,16 @@ struct SampleParams {
     double temperature_all, top_p_all, min_p_all;
     int32_t top_k_all;
     uint32_t vocab;
-    int scale_bits;
+    int scale_bits, limb_bits;
     int64_t *tokens;
     float *probs;
 };
 
+// Masses in three limbs of `limb_bits`, which a block's sums of cannot
+// overflow: three additions whose results nobody waits for, in any order.
+// Counts are in the first.
 struct Histogram {
-    uint32_t low[kBins], high[kBins];  // 64-bit masses, or counts in `low`
+    uint32_t limb[3][kBins];
 };
 
 // Everything that is kept: logits above `value`, and the first `ties` equal to it.
@@ -86,12 +89,11 @@ struct SampleShared {
     uint64_t found_above, found_in;
 };
 
-// Adds a 64-bit mass by two 32-bit atomics, whose order changes nothing.
-__device__ __forceinline__ void add_mass(Histogram &h, uint32_t bin, uint64_t mass) {
-    const uint32_t low = (uint32_t)mass;
-    const uint32_t old = atomicAdd(&h.low[bin], low);
-    const uint32_t high = (uint32_t)(mass >> 32) + (old + low < old);
-    if (high) atomicAdd(&h.high[bin], high);
+__device__ __forceinline__ void add_mass(Histogram &h, uint32_t bin, uint64_t mass, int limb_bits) {
+    const uint32_t mask = (1u << limb_bits) - 1;
+    atomicAdd(&h.limb[0][bin], (uint32_t)mass & mask);
+    atomicAdd(&h.limb[1][bin], (uint32_t)(mass >> limb_bits) & mask);
+    atomicAdd(&h.limb[2][bin], (uint32_t)(mass >> 2 * limb_bits));
 }
 
 __device__ __forceinline__ uint64_t warp_scan(uint64_t v) {  // inclusive
@@ -220,11 +222,11 @@ struct Weigher {
     float max, floor;  // floor: a lower logit has no mass
     float top, slope32;  // max, or the largest finite number; slope in 32 bits
     double slope;        // 16 log2(e) / T
-    int scale_bits;
+    int scale_bits, limb_bits;
     const double *roots;  // kRoots in shared memory
 
-    __device__ Weigher(float max_, double t, int scale_bits_, const double *roots_)
-        : max(max_), scale_bits(scale_bits_), roots(roots_) {
+    __device__ Weigher(float max_, double t, int scale_bits_, int limb_bits_, const double *roots_)
+        : max(max_), scale_bits(scale_bits_), limb_bits(limb_bits_), roots(roots_) {
         top = fminf(max, FLT_MAX);
         slope = 16 * 1.4426950408889634 / t;
         slope32 = (float)slope;
@@ -301,11 +303,11 @@ template <typename N> __device__ __forceinline__ N sum_over_blocks(const N &of, 
 
 __device__ __noinline__ void mass_to_bin(const Weigher &weigh, Histogram &h, uint32_t bin, float l) {
     const uint64_t mass = weigh.mass_or_none(l);
-    if (mass) add_mass(h, bin, mass);
+    if (mass) add_mass(h, bin, mass, weigh.limb_bits);
 }
 
 __device__ __forceinline__ void clear(Histogram &h) {
-    for (int i = threadIdx.x; i < kBins; i += kSampleThreads) h.low[i] = h.high[i] = 0;
+    for (int i = threadIdx.x; i < kBins; i += kSampleThreads) h.limb[0][i] = h.limb[1][i] = h.limb[2][i] = 0;
     __syncthreads();
 }
 
@@ -313,24 +315,26 @@ __device__ __forceinline__ void clear(Histogram &h) {
 // at which `before` plus the running sum reaches `wanted(all)` (kBins: none),
 // what it holds, and the sum before it; the same for every block.
 template <bool MASS, typename Wanted>
-__device__ uint32_t find_bin(Histogram &h, SampleShared &s, uint64_t before, Wanted &&wanted) {
+__device__ uint32_t find_bin(Histogram &h, SampleShared &s, int limb_bits, uint64_t before, Wanted &&wanted) {
     const cg::cluster_group cluster = cg::this_cluster();
     using Bins = Pack<uint32_t, kBinsPerThread>;
     const uint32_t t = threadIdx.x;
     uint64_t bins[kBinsPerThread] = {}, sum = 0, all;
-    Bins lo[kMaxCluster] = {}, hi[kMaxCluster] = {};
 #pragma unroll
-    for (uint32_t b = 0; b < kMaxCluster; ++b) {
-        if (b < cluster.num_blocks()) {
-            const Histogram *o = cluster.map_shared_rank(&h, b);
-            lo[b] = *reinterpret_cast<const Bins *>(&o->low[t * kBinsPerThread]);
-            if (MASS) hi[b] = *reinterpret_cast<const Bins *>(&o->high[t * kBinsPerThread]);
+    for (int limb = 0; limb < (MASS ? 3 : 1); ++limb) {
+        Bins theirs[kMaxCluster] = {};
+#pragma unroll
+        for (uint32_t b = 0; b < kMaxCluster; ++b)
+            if (b < cluster.num_blocks())
+                theirs[b] = *reinterpret_cast<const Bins *>(&cluster.map_shared_rank(&h, b)->limb[limb][t * kBinsPerThread]);
+#pragma unroll
+        for (int i = 0; i < kBinsPerThread; ++i) {
+            uint64_t of = 0;
+#pragma unroll
+            for (int b = 0; b < kMaxCluster; ++b) of += theirs[b].e[i];
+            bins[i] += of << limb * limb_bits;
         }
     }
-#pragma unroll
-    for (int b = 0; b < kMaxCluster; ++b)
-#pragma unroll
-        for (int i = 0; i < kBinsPerThread; ++i) bins[i] += (uint64_t)hi[b].e[i] << 32 | lo[b].e[i];
 #pragma unroll
     for (int i = 0; i < kBinsPerThread; ++i) sum += bins[i];
     if (t == 0) s.found_bin = kBins;
@@ -402,14 +406,14 @@ __device__ Narrowed narrow(const RowPart<T> &part, const Weigher &weigh, SampleS
                     bin = (high - ordered_number(l)) >> shift;
                 }
                 if constexpr (MASS) mass_to_bin(weigh, h, bin, l);
-                else atomicAdd(&h.low[bin], 1u);
+                else atomicAdd(&h.limb[0][bin], 1u);
             }
         });
         cluster.sync();
         // The other histogram is cleared next, after this barrier, when no
         // block reads it any more.
         uint64_t total = 0;
-        const uint32_t bin = find_bin<MASS>(h, s, got.above, [&](uint64_t all) {
+        const uint32_t bin = find_bin<MASS>(h, s, weigh.limb_bits, got.above, [&](uint64_t all) {
             total = all;
             if (shift < 0) got.wanted = need(all);
             return got.wanted;
@@ -656,7 +660,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     }
 
     t = fmax(t, 0x1p-100);  // 1 / t stays a number in 32 bits
-    const Weigher weigh(max, t, p.scale_bits, s.roots);
+    const Weigher weigh(max, t, p.scale_bits, p.limb_bits, s.roots);
     const double least_w = min_p > 0.0 ? fmin(min_p, 1.0) : 0.0;
     const uint64_t least = (uint64_t)ceil(least_w * (double)(1ull << p.scale_bits));
     // top-k: the distance from the mean to the maximum covers every k below
@@ -690,10 +694,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                 if (!(largest(v) >= edge)) return;
 #pragma unroll
                 for (int j = 0; j < RowPart<T>::V; ++j)
-                    if (v[j] >= edge) atomicAdd(&h.low[steps.bin(v[j])], 1u);
+                    if (v[j] >= edge) atomicAdd(&h.limb[0][steps.bin(v[j])], 1u);
             });
             cluster.sync();
-            last = find_bin<false>(h, s, 0, [&](uint64_t) { return (uint64_t)k; });
+            last = find_bin<false>(h, s, 0, 0, [&](uint64_t) { return (uint64_t)k; });
             if (last < kBins - 1) located = {last, s.found_above, (uint64_t)k};
             fits = located.bin < kBins && s.found_above + s.found_in <= kListed;
         } else {
@@ -702,30 +706,32 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                 uint64_t x, y;
                 weigh.masses(a, b, weigh.floor, x, y);
                 mass += x + y;
-                if (a >= edge) add_mass(h, steps.bin(a), x);
-                if (b >= edge) add_mass(h, steps.bin(b), y);
+                if (a >= edge) add_mass(h, steps.bin(a), x, weigh.limb_bits);
+                if (b >= edge) add_mass(h, steps.bin(b), y, weigh.limb_bits);
             });
             uint64_t mine;
             block_scan(mass, s, mine);
             if (threadIdx.x == 0) s.block_mass = mine;
             cluster.sync();
             whole = (uint64_t)sum_over_blocks((int64_t &)s.block_mass, blocks);
-            last = find_bin<true>(h, s, 0, [&](uint64_t) { return part_of(whole, top_p); });
+            last = find_bin<true>(h, s, weigh.limb_bits, 0, [&](uint64_t) { return part_of(whole, top_p); });
             fits = last < kBins - 1;
             if (fits) located = {last, s.found_above, part_of(whole, top_p)};
         }
         if (fits || located.bin < kBins) {
             // Two lists: of all that may be kept, and of the last step alone.
-            const float from = steps.below(last);
+            const float from = steps.below(last), above = steps.above(last);
             part.each([&](const float(&v)[RowPart<T>::V], uint32_t index) {
                 if (!(largest(v) >= from)) return;
+                // Past its end the first list is of no use, and a common counter slow.
+                const bool both = fits && *(volatile uint32_t *)&s.listed[0] <= kListed;
+                const float upto = both ? INFINITY : above;
 #pragma unroll
                 for (int j = 0; j < RowPart<T>::V; ++j) {
-                    if (!(v[j] >= from)) continue;
+                    if (!(v[j] >= from && v[j] <= upto)) continue;
                     const uint32_t bin = steps.bin(v[j]);
                     const uint64_t entry = (uint64_t)~ordered_number(v[j]) << 32 | (index + j);
-                    // (Past its end the list is of no use, and a common counter slow.)
-                    if (fits && bin <= last && *(volatile uint32_t *)&s.listed[0] <= kListed) {
+                    if (both && bin <= last) {
                         const uint32_t at = atomicAdd(&s.listed[0], 1u);
                         if (at < kListed) s.list[at] = entry;
                     }
@@ -873,10 +879,12 @@ heph_status launch_sample(const SampleArgs &a, int sm_count, cudaStream_t stream
     while (blocks < kMaxCluster && (((uint64_t)a.rows * blocks * 2 <= (uint32_t)sm_count && a.vocab / (blocks * 2) >= 4096) ||
                                     a.vocab / blocks >= 65536))
         blocks *= 2;
-    // vocab x 2^scale_bits stays below 2^62, and a mass below 2^52.
-    const int bits = 32 - __builtin_clz(a.vocab);
+    // vocab x 2^scale_bits stays below 2^62, a mass below that of three limbs,
+    // and the sum of a limb of a block's logits (an eighth of the row and 4096,
+    // or less than 2^17) below 2^32.
+    const int bits = 32 - __builtin_clz(a.vocab), limb_bits = a.vocab <= (1u << 20) - (1u << 16) ? 15 : 13;
     const SampleParams p{a.logits.ptr, a.logits.stride, a.uniform, a.temperature, a.top_p, a.min_p, a.top_k,
-                         a.temperature_all, a.top_p_all, a.min_p_all, a.top_k_all, a.vocab, std::min(50, 62 - bits),
+                         a.temperature_all, a.top_p_all, a.min_p_all, a.top_k_all, a.vocab, std::min(3 * limb_bits - 1, 62 - bits), limb_bits,
                          a.tokens, a.probs};
     return dispatch_row_dtype(a.dtype, [&]<typename T>() -> heph_status {
         return launch_clusters("token sampling", sample_kernel<T>, dim3(a.rows * blocks), dim3(kSampleThreads), blocks, 0,

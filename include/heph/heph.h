@@ -557,7 +557,7 @@ heph_status heph_expert_order(int ordinal, const int32_t *picks, uint64_t count,
                               int32_t *offsets, int32_t *order, int32_t *slot, void *workspace,
                               uint64_t workspace_bytes, heph_stream stream);
 
-/* Draws a token from every row of `logits`: w_i = exp((l_i - max l) / T).  In
+/* Draws a token from every row of `logits` (up to 2^22 - 2^16 wide): w_i = exp((l_i - max l) / T).  In
  * the order of falling l (lowest index first among equals) top_k keeps the
  * first k (0: off), top_p of those the ones before which lies less than top_p
  * of their mass (1: off), min_p of those the ones with w >= min_p (0: off);
