@@ -411,7 +411,8 @@ route_kernel(const __grid_constant__ RouteParams p) {
             least = __reduce_max_sync(kFullMask, head);
             if (head == least) head = 0;
         }
-        if (least && !exact) least = ordered_number(key_value(least) - 2.0f * margin(key_value(least))) & ~kLow;
+        const float bound = key_value(least) - 2.0f * margin(key_value(least));
+        if (least && !exact && bound == bound) least = ordered_number(bound) & ~kLow;  // (+inf is its own bound)
         least = max(least, 1u);
 #pragma unroll
         for (int j = 0; j < N; ++j) {

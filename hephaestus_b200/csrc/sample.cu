@@ -872,9 +872,9 @@ heph_status launch_sample(const SampleArgs &a, int sm_count, cudaStream_t stream
     // A row's blocks (a cluster) share its passes: as many as there are SMs
     // for all rows, while each still has some work; and, as rows may differ
     // much in theirs, never over a share of 64 K logits each.  Measured on one
-    // B200 with 1 / 2 / 4 / 8 blocks a row: 1 row of 131072 43 / 30 / 24 / 21
-    // us, 128 of 50257 28.7 / 32 / 46 / 69, 256 of 131072, each with settings
-    // of its own, 280 / 192 / 179 / 228.
+    // B200 with 1 / 2 / 4 / 8 blocks a row: 1 row of 131072 41 / 29 / 22 / 21
+    // us, 128 of 50257 27 / 31 / 43 / 65, 256 of 131072, each with settings of
+    // its own, 233 / 173 / 167 / 226.
     uint32_t blocks = 1;
     while (blocks < kMaxCluster && (((uint64_t)a.rows * blocks * 2 <= (uint32_t)sm_count && a.vocab / (blocks * 2) >= 4096) ||
                                     a.vocab / blocks >= 65536))

@@ -102,6 +102,11 @@ void check_grad(const char *name, const at::Tensor &t) {
         refuse(std::string(name) + " asks for a gradient, which these calls do not record: detach it, or use torch.no_grad()");
 }
 
+// What the tensor holds is what its memory says.
+void check_plain(const char *name, const at::Tensor &t) {
+    if (t.layout() != at::kStrided || t.is_neg()) refuse(std::string(name) + " must be a strided tensor of plain values");
+}
+
 // A tensor as rows of adjacent columns.
 struct Matrix {
     const void *ptr = nullptr;
@@ -118,7 +123,7 @@ Matrix rows_of(const char *name, const at::Tensor &t, at::ScalarType dtype = at:
     } else if (have != dtype) {
         refuse(std::string(name) + " must be " + dtype_name(dtype) + ", not " + dtype_name(have));
     }
-    if (t.layout() != at::kStrided) refuse(std::string(name) + " must be a strided tensor");
+    check_plain(name, t);
     const at::IntArrayRef sizes = t.sizes(), strides = t.strides();
     if (shape && sizes != *shape) refuse(std::string(name) + " has shape " + text(sizes) + ", not " + text(*shape));
     const int64_t dims = t.dim();
@@ -138,6 +143,7 @@ Matrix rows_of(const char *name, const at::Tensor &t, at::ScalarType dtype = at:
             upto *= sizes[d];
         }
     }
+    if (m.rows <= 1) m.stride = m.cols;  // one row: as good as contiguous
     check_grad(name, t);
     m.ptr = t.const_data_ptr();
     return m;
@@ -151,7 +157,8 @@ const void *vector_of(const char *name, const at::Tensor &t, int64_t length, std
         for (const at::ScalarType d : dtypes) names += (names.empty() ? "" : " or ") + std::string(dtype_name(d));
         refuse(std::string(name) + " must be " + names + ", not " + dtype_name(t.scalar_type()));
     }
-    if (t.layout() != at::kStrided || t.dim() != 1 || t.size(0) != length || (t.stride(0) != 1 && length > 1))
+    check_plain(name, t);
+    if (t.dim() != 1 || t.size(0) != length || (t.stride(0) != 1 && length > 1))
         refuse(std::string(name) + " must be a vector of " + std::to_string(length) + " adjacent elements");
     check_grad(name, t);
     return t.const_data_ptr();
@@ -340,7 +347,8 @@ PyObject *route_experts_backward(PyObject *const *args) {
 PyObject *expert_order(PyObject *const *args) {
     const at::Tensor &experts = tensor(args[0], "experts");
     if (experts.scalar_type() != at::kInt) refuse(std::string("experts must be torch.int32, not ") + dtype_name(experts.scalar_type()));
-    if (experts.layout() != at::kStrided || !experts.is_contiguous()) refuse("experts must be contiguous");
+    check_plain("experts", experts);
+    if (!experts.is_contiguous()) refuse("experts must be contiguous");
     const int64_t num = whole(args[1], "num_experts", INT64_MIN, INT64_MAX);
     if (num < 1 || num > 1024) refuse("expert_order takes 1 to 1024 experts, not " + std::to_string(num));
     const int device = device_of({&experts});

@@ -37,6 +37,11 @@ def test_norm_refusals():
     refused("dy has shape", T.rms_norm_backward, X[:1], X)
     refused("s must have", T.rms_norm_backward, X.t(), X.t())
     refused("must be a torch tensor", T.rms_norm, None)
+    refused("plain values", T.rms_norm, torch._neg_view(X))
+    refused("plain values", T.rms_norm, X, torch._neg_view(X[0]))
+    refused("plain values", T.rms_norm, X.to_sparse())
+    with torch.no_grad():  # nothing is recorded: the device is asked for next
+        refused("needs CUDA tensors", T.rms_norm, X, torch.zeros(64, requires_grad=True))
     refused("needs CUDA tensors", T.rms_norm, X, torch.zeros(64))
 
 

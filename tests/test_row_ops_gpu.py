@@ -184,7 +184,8 @@ def test_route(T, dtype, rows, experts, k):
 
 
 @pytest.mark.parametrize("experts,groups,kept,k", [(8, 8, 3, 3), (12, 3, 2, 5), (16, 4, 4, 16), (64, 8, 4, 6),
-                                                   (256, 8, 4, 8), (96, 32, 7, 8), (520, 4, 1, 20), (1024, 16, 3, 8)])
+                                                   (256, 8, 4, 8), (96, 32, 7, 8), (520, 4, 1, 20), (1024, 16, 3, 8),
+                                                   (256, 8, 1, 8), (256, 8, 2, 8), (128, 4, 1, 16), (300, 4, 3, 8)])
 def test_route_groups(T, experts, groups, kept, k):
     logits = rand(77, experts, seed=experts)
     bias = rand(experts, seed=3, scale=0.3)
@@ -207,6 +208,36 @@ def test_route_ties_go_to_the_lowest_index(T):
     _, picks = check_route(T, close, 2, score="sigmoid")
     assert picks[0].tolist() == [40, 0]
     check_route(T, close, 2, score="sigmoid", bias=torch.full((64,), 0.5, device="cuda"))
+
+
+@pytest.mark.parametrize("experts", [32, 60, 256, 700])
+def test_route_near_sums(T, experts):
+    """Every score + bias within 1e-7 of the others: what 32 bits cannot tell apart, 64 bits do."""
+    logits = rand(1, experts, seed=experts).expand(3, experts)
+    for score, s in (("sigmoid", torch.sigmoid(logits[0].double())), ("softmax", torch.softmax(logits[0].double(), 0))):
+        bias = (1.0 - s).float()
+        for k in (1, 8, 12, 13, 32):
+            check_route(T, logits, k, score=score, bias=bias)
+        check_route(T, logits, 8, score=score, bias=bias, groups=4, groups_kept=2)
+        check_route(T, logits, 3, score=score, bias=bias, groups={32: 8, 60: 15, 256: 32, 700: 20}[experts],
+                    groups_kept=3, group_top=1)
+    # Logits a unit apart, and equal ones.
+    close = torch.full((2, experts), 1.0, device="cuda")
+    for at in (3, 17, experts - 1):
+        close[:, at] = torch.nextafter(close[0, at], torch.tensor(2.0, device="cuda"))
+    for k in (1, 2, 5, 20):
+        check_route(T, close, k)
+        check_route(T, close, k, score="sigmoid", groups=4, groups_kept=3)
+
+
+def test_route_infinite_bias(T):
+    logits, bias = rand(5, 64, seed=1), torch.zeros(64, device="cuda")
+    bias[[4, 9, 33]] = float("inf")
+    for k in (1, 2, 3, 6):
+        for kw in (dict(), dict(score="sigmoid"), dict(groups=8, groups_kept=2)):
+            _, picks = check_route(T, logits, k, bias=bias, **kw)
+            if not kw.get("groups"):
+                assert picks[0].tolist()[:3] == [4, 9, 33][:k]
 
 
 def test_route_masked_and_special(T):
@@ -427,6 +458,29 @@ def test_sample_scales_of_logits(T):
             for kw in (dict(top_k=100), dict(top_k=19999), dict(top_p=0.6), dict(top_p=0.6, temperature=1e3),
                        dict(top_k=3000, top_p=0.3, temperature=scale)):
                 check_sample(T, x * scale + shift, u, **kw)
+
+
+def test_sample_wide_rows(T):
+    """Vocabularies past 2^20 (masses in shorter limbs), and the widest."""
+    for vocab in (1000000, 1100003, (1 << 22) - (1 << 16)):
+        logits = rand(2, vocab, seed=vocab, scale=2)
+        u = torch.tensor([0.3, 0.97], device="cuda")
+        for kw in (dict(), dict(top_k=700), dict(top_p=0.01), dict(top_p=0.9, temperature=1.3), dict(top_k=5000, top_p=0.5)):
+            check_sample(T, logits, u, **kw)
+    # All equal: the most that a bin can hold.
+    flat = torch.zeros(2, 1100003, device="cuda")
+    check_sample(T, flat, u, top_p=0.7)
+    check_sample(T, flat, u, top_k=600000, top_p=0.7)
+
+
+def test_sample_tiny_temperatures(T):
+    logits = rand(4, 5000, seed=8)
+    logits[:, 100] = logits[:, 4000] = 9.0
+    u = torch.tensor([0.1, 0.49, 0.51, 0.9], device="cuda")
+    for t in (1e-3, 1e-20, 1e-38, 1e-300):
+        for kw in (dict(), dict(top_p=0.4), dict(top_k=3)):
+            tokens = check_sample(T, logits, u, temperature=t, **kw)
+    assert tokens.tolist() == [100, 100, 4000, 4000]
 
 
 def test_sample_numbers_outside_the_range(T):
