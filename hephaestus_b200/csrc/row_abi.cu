@@ -185,7 +185,7 @@ extern "C" heph_status heph_rms_norm_backward_workspace(int ordinal, uint64_t ro
         if (rows > kMaxRows || cols > kMaxCols) return refuse("rms_norm_backward rows or columns out of range");
         int sms = 0;
         HEPH_TRY(sm_count(ordinal, &sms));
-        *out_bytes = (uint64_t)norm_grad_partials((uint32_t)rows, sms) * cols * sizeof(float);
+        *out_bytes = (uint64_t)norm_grad_partials((uint32_t)rows, (uint32_t)cols, sms) * cols * sizeof(float);
         return HEPH_OK;
     });
 }
@@ -214,7 +214,7 @@ extern "C" heph_status heph_rms_norm_backward(int ordinal, heph_row_dtype dtype,
         HEPH_TRY(on.enter(ordinal));
         int sms = 0;
         HEPH_TRY(sm_count(ordinal, &sms));
-        const uint64_t need = dweight ? (uint64_t)norm_grad_partials((uint32_t)rows, sms) * cols * sizeof(float) : 0;
+        const uint64_t need = dweight ? (uint64_t)norm_grad_partials((uint32_t)rows, (uint32_t)cols, sms) * cols * sizeof(float) : 0;
         if (need && (!workspace || workspace_bytes < need))
             return refuse("rms_norm_backward needs a workspace of " + std::to_string(need) + " bytes");
         return launch_rms_norm_backward({dtype, {dy, dy_stride}, {x, x_stride}, {dsum, dsum_stride}, weight,

@@ -10,6 +10,9 @@
 // All in 32 bits from the unrounded sum s; each output is rounded once.
 #include <cuda_fp8.h>
 
+#include <algorithm>
+#include <initializer_list>
+
 #include "row_ops.h"
 #include "row_utils.cuh"
 
@@ -115,13 +118,124 @@ __device__ __forceinline__ void shared_max(float *at, float v) {
 }
 __device__ __forceinline__ float scale_of(float amax) { return fmaxf(amax, kFp8Floor) * (1.0f / kFp8Max); }
 
+// Columns of a thread's chunks of V, `step` apart.  SHIFTED: rows of odd widths.
+// Row r of every operand starts the same number of elements past a 16-byte
+// boundary, `lead`; chunks go from boundary to boundary, and the row's two
+// ends, which are parts of chunks, are taken element by element.
+template <int V, int C, bool SHIFTED> struct Chunks {
+    uint32_t cols, step, origin;
+    uint32_t wholes = 0, somes = 0;  // chunks that lie in the row, and of which some column does, a bit each
+    __device__ Chunks(uint32_t cols_, const void *row, size_t size)
+        : cols(cols_), step(blockDim.x * V),
+          origin(threadIdx.x * V - (SHIFTED ? (uint32_t)((reinterpret_cast<uintptr_t>(row) & 15u) / size) : 0)) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const uint32_t col = first(c);
+            wholes |= (col < cols && (!SHIFTED || col + V <= cols) ? 1u : 0u) << c;
+            somes |= (SHIFTED ? col + V - 1 < cols + V - 1 : col < cols ? 1u : 0u) << c;
+        }
+    }
+    // Chunk c's first column; a SHIFTED row's first chunk starts before column
+    // 0, and the number wraps.
+    __device__ __forceinline__ uint32_t first(int c) const { return c * step + origin; }
+    __device__ __forceinline__ bool whole(int c) const { return wholes >> c & 1u; }
+    __device__ __forceinline__ bool some(int c) const { return somes >> c & 1u; }
+    __device__ __forceinline__ bool has(uint32_t col, int j) const { return !SHIFTED || col + j < cols; }
+
+    template <typename T> __device__ __forceinline__ Pack<T, V> load(const T *row, int c) const {
+        const uint32_t col = first(c);
+        if (!SHIFTED || whole(c)) return *reinterpret_cast<const Pack<T, V> *>(row + col);
+        Pack<T, V> u;
+#pragma unroll
+        for (int j = 0; j < V; ++j) u.e[j] = has(col, j) ? row[col + j] : from_f32<T>(0.0f);
+        return u;
+    }
+    template <typename T> __device__ __forceinline__ void store(T *row, int c, const float (&v)[V]) const {
+        const uint32_t col = first(c);
+        if (!SHIFTED || whole(c)) {
+            store_as<T, V>(row + col, v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (has(col, j)) row[col + j] = from_f32<T>(v[j]);
+        }
+    }
+    // V weights; those of SHIFTED chunks have their boundaries elsewhere.
+    template <typename T> __device__ __forceinline__ void weights(const void *weight, bool f32, int c, float (&w)[V]) const {
+        const uint32_t col = first(c);
+        if constexpr (!SHIFTED) {
+            load_weight<T, V>(weight, f32, col, w);
+        } else if (!weight) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) w[j] = 1.0f;
+        } else {
+            const bool all = whole(c);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                float one[1] = {0.0f};
+                if (all || has(col, j)) load_weight<T, 1>(weight, f32, col + j, one);
+                w[j] = one[0];
+            }
+        }
+    }
+};
+
+// The end of a row: from w s in v, the sum of s^2 and the maxima of |w s| to
+// the outputs.
+template <typename T, int V, int C, Scales S, bool SHIFTED>
+__device__ __forceinline__ void finish_row(const NormParams &p, uint32_t row, const Chunks<V, C, SHIFTED> &chunks, float (&v)[C][V], float ss,
+                                           float amax, const float (&gmax)[C], const float *group_max) {
+    const float rstd = rsqrtf(ss * p.per_col + p.eps);
+    // |w s| rstd rounds monotonically, so the maximum of |y| is the rounded
+    // product of the maximum of |w s|.
+    float scale, factor = rstd;
+    if (S == kRowScale) {
+        scale = scale_of(amax * rstd);
+        factor = rstd * __fdividef(1.0f, scale);
+        if (threadIdx.x == 0) p.scales[row] = scale;
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const uint32_t col = chunks.first(c);
+        if (!chunks.some(c)) continue;
+        if (S == kLaneScales || (S == kSharedScales && !SHIFTED)) {
+            const uint32_t g = col >> p.group_shift;
+            scale = scale_of((S == kLaneScales ? gmax[c] : group_max[g]) * rstd);
+            factor = rstd * __fdividef(1.0f, scale);
+            if (col == g << p.group_shift) p.scales[(int64_t)row * p.groups + g] = scale;
+        }
+        if (S == kSharedScales && SHIFTED) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if (!chunks.has(col, j)) continue;
+                const uint32_t g = (col + j) >> p.group_shift;
+                scale = scale_of(group_max[g] * rstd);
+                v[c][j] *= rstd * __fdividef(1.0f, scale);
+                if (col + j == g << p.group_shift) p.scales[(int64_t)row * p.groups + g] = scale;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[c][j] *= factor;
+        }
+        if constexpr (S == kNoScales) {
+            chunks.store(static_cast<T *>(p.y) + (int64_t)row * p.cols, c, v[c]);
+        } else {
+            uint8_t *q = static_cast<uint8_t *>(p.y) + (int64_t)row * p.cols;
+            if (!SHIFTED) {
+                store_fp8<V>(q + col, v[c]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float one[1] = {v[c][j]};
+                    if (chunks.has(col, j)) store_fp8<1>(q + (col + j), one);
+                }
+            }
+        }
+    }
+}
+
 // A row (or, blockDim.y > 1, a row per warp) whose C x V values per thread
 // stay in registers between the one read and the one write.
-//
-// SHIFTED: rows of odd widths.  Row r of every operand starts the same number
-// of elements past a 16-byte boundary; accesses are whole vectors from
-// boundary to boundary, but for the row's two ends (and the weights, whose
-// boundaries are elsewhere: element by element, from L1).
 template <typename T, int V, int C, Scales S, bool RES, bool SHIFTED>
 __global__ void __launch_bounds__(C * V >= 32 ? 512 : 1024) norm_kernel(const __grid_constant__ NormParams p) {
     extern __shared__ float group_max[];  // kSharedScales: of each group
@@ -129,72 +243,40 @@ __global__ void __launch_bounds__(C * V >= 32 ? 512 : 1024) norm_kernel(const __
     const bool warp_rows = blockDim.y > 1;
     const uint32_t row = blockIdx.x * blockDim.y + threadIdx.y;
     if (row >= p.rows) return;  // whole warps, which no block barrier waits for
-    const uint32_t t = threadIdx.x, step = blockDim.x * V;
     const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
     const T *res = RES ? static_cast<const T *>(p.residual) + row * p.residual_stride : nullptr;
-    T *sum = RES ? static_cast<T *>(p.sum) + (int64_t)row * p.cols : nullptr;
-    // Columns of this thread's chunk c: first, first + 1, ...; a SHIFTED row's
-    // first chunk starts before column 0 (and the unsigned number wraps).
-    const uint32_t lead = SHIFTED ? (uint32_t)(reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T) : 0;
-    auto first = [&](int c) { return c * step + t * V - lead; };
-    auto whole = [&](uint32_t col) { return SHIFTED ? col < p.cols && col + V <= p.cols : col < p.cols; };
-    auto some = [&](uint32_t col) { return SHIFTED && col + V - 1 < p.cols + V - 1; };  // part of it, or all
+    const Chunks<V, C, SHIFTED> chunks(p.cols, x, sizeof(T));
     if (S == kSharedScales) {
-        for (uint32_t g = t; g < p.groups; g += blockDim.x) group_max[g] = 0.0f;
+        for (uint32_t g = threadIdx.x; g < p.groups; g += blockDim.x) group_max[g] = 0.0f;
         __syncthreads();
     }
 
     Pack<T, V> ux[C], ur[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        const uint32_t col = first(c);
-        if (whole(col)) {
-            ux[c] = *reinterpret_cast<const Pack<T, V> *>(x + col);
-            if (RES) ur[c] = *reinterpret_cast<const Pack<T, V> *>(res + col);
-        } else if (some(col)) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                ux[c].e[j] = col + j < p.cols ? x[col + j] : from_f32<T>(0.0f);
-                if (RES) ur[c].e[j] = col + j < p.cols ? res[col + j] : from_f32<T>(0.0f);
-            }
+        const uint32_t col = chunks.first(c);
+        if (chunks.some(c)) {
+            ux[c] = chunks.load(x, c);
+            if (RES) ur[c] = chunks.load(res, c);
         }
     }
     float v[C][V], ss = 0.0f, amax = 0.0f, gmax[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        const uint32_t col = first(c);
+        const uint32_t col = chunks.first(c);
         gmax[c] = 0.0f;
-        if (whole(col) || some(col)) {
+        if (chunks.some(c)) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 v[c][j] = to_f32(ux[c].e[j]);
                 if (RES) v[c][j] += to_f32(ur[c].e[j]);
                 ss += v[c][j] * v[c][j];
             }
-            if (RES) {
-                if (whole(col)) {
-                    store_as<T, V>(sum + col, v[c]);
-                } else {
+            if (RES) chunks.store(static_cast<T *>(p.sum) + (int64_t)row * p.cols, c, v[c]);
+            float w[V];
+            chunks.template weights<T>(p.weight, p.weight_f32, c, w);
 #pragma unroll
-                    for (int j = 0; j < V; ++j)
-                        if (col + j < p.cols) sum[col + j] = from_f32<T>(v[c][j]);
-                }
-            }
-            if (SHIFTED) {
-                if (p.weight) {
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        float w[1] = {0.0f};
-                        if (col + j < p.cols) load_weight<T, 1>(p.weight, p.weight_f32, col + j, w);
-                        v[c][j] *= w[0];
-                    }
-                }
-            } else {
-                float w[V];
-                load_weight<T, V>(p.weight, p.weight_f32, col, w);
-#pragma unroll
-                for (int j = 0; j < V; ++j) v[c][j] *= w[j];
-            }
+            for (int j = 0; j < V; ++j) v[c][j] *= w[j];
             if (S == kRowScale || S == kLaneScales || (S == kSharedScales && !SHIFTED)) {
 #pragma unroll
                 for (int j = 0; j < V; ++j) gmax[c] = fmaxf(gmax[c], fabsf(v[c][j]));
@@ -206,7 +288,7 @@ __global__ void __launch_bounds__(C * V >= 32 ? 512 : 1024) norm_kernel(const __
                 float a = 0.0f, b = 0.0f;
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    const bool next = col + j < p.cols && (col + j) >> p.group_shift != g;
+                    const bool next = chunks.has(col, j) && (col + j) >> p.group_shift != g;
                     a = fmaxf(a, next ? 0.0f : fabsf(v[c][j]));
                     b = fmaxf(b, next ? fabsf(v[c][j]) : 0.0f);
                 }
@@ -220,57 +302,7 @@ __global__ void __launch_bounds__(C * V >= 32 ? 512 : 1024) norm_kernel(const __
     }
     row_fold<S == kRowScale, true>(ss, amax, warp_rows, red);
     if (S == kSharedScales) __syncthreads();
-    const float rstd = rsqrtf(ss * p.per_col + p.eps);
-    // |w s| rstd rounds monotonically, so the maximum of |y| is the rounded
-    // product of the maximum of |w s|.
-    float scale, factor = rstd;
-    if (S == kRowScale) {
-        scale = scale_of(amax * rstd);
-        factor = rstd * __fdividef(1.0f, scale);
-        if (t == 0) p.scales[row] = scale;
-    }
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const uint32_t col = first(c);
-        if (!whole(col) && !some(col)) continue;
-        const int64_t at = (int64_t)row * p.cols + (int32_t)col;
-        if (S == kLaneScales || (S == kSharedScales && !SHIFTED)) {
-            const uint32_t g = col >> p.group_shift;
-            scale = scale_of((S == kLaneScales ? gmax[c] : group_max[g]) * rstd);
-            factor = rstd * __fdividef(1.0f, scale);
-            if (col == g << p.group_shift) p.scales[(int64_t)row * p.groups + g] = scale;
-        }
-        if (S == kSharedScales && SHIFTED) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                if (col + j >= p.cols) continue;
-                const uint32_t g = (col + j) >> p.group_shift;
-                scale = scale_of(group_max[g] * rstd);
-                v[c][j] *= rstd * __fdividef(1.0f, scale);
-                if (col + j == g << p.group_shift) p.scales[(int64_t)row * p.groups + g] = scale;
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) v[c][j] *= factor;
-        }
-        if constexpr (S != kNoScales) {
-            if (!SHIFTED) {
-                store_fp8<V>(static_cast<uint8_t *>(p.y) + at, v[c]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float one[1] = {v[c][j]};
-                    if (col + j < p.cols) store_fp8<1>(static_cast<uint8_t *>(p.y) + at + j, one);
-                }
-            }
-        } else if (whole(col)) {
-            store_as<T, V>(static_cast<T *>(p.y) + at, v[c]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (col + j < p.cols) static_cast<T *>(p.y)[at + j] = from_f32<T>(v[c][j]);
-        }
-    }
+    finish_row<T, V, C, S, SHIFTED>(p, row, chunks, v, ss, amax, gmax, group_max);
 }
 
 // Rows too long for the registers, or of operands with no common boundaries:
@@ -342,7 +374,7 @@ template <typename T, int V, bool FP8> __global__ void __launch_bounds__(1024) n
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool aligned_rows(const Rows &r, size_t es) { return aligned16(r.ptr) && (r.stride * (int64_t)es) % 16 == 0; }
 
-// SHIFTED (see norm_kernel) or not: rows of whole vectors.
+// SHIFTED (see Chunks) or not: rows of whole vectors.
 template <typename T, bool FP8, bool SHIFTED> heph_status launch_norm(const NormParams &p, cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
     constexpr int kMost = 32 / V;  // chunks of a thread: 32 registers
@@ -352,14 +384,15 @@ template <typename T, bool FP8, bool SHIFTED> heph_status launch_norm(const Norm
     // wait less for one another.
     uint32_t c = 1;
     while (c < kMost && (units + c - 1) / c > 256) c *= 2;
+    const bool in_lanes = !SHIFTED && p.groups > 1 && (1u << p.group_shift) / V <= 32;
+    const bool own_scales = !FP8 || p.groups == 1 || in_lanes;  // no group_max
     const uint32_t threads = ((units + c - 1) / c + 31) / 32 * 32;
     if (threads > (c * V >= 32 ? 512 : 1024)) {
         if constexpr (!SHIFTED) return launch_rows("long row norm", norm_long_kernel<T, V, FP8>, dim3(p.rows), dim3(1024), smem, stream, p);
         return launch_rows("long row norm", norm_long_kernel<T, 1, FP8>, dim3(p.rows), dim3(1024), smem, stream, p);
     }
-    const bool in_lanes = !SHIFTED && p.groups > 1 && (1u << p.group_shift) / V <= 32;
     // Short rows: one warp each, eight to a block (not where they share group_max).
-    const uint32_t per_block = threads == 32 && (!FP8 || p.groups == 1 || in_lanes) ? 8 : 1;
+    const uint32_t per_block = threads == 32 && own_scales ? 8 : 1;
     const dim3 grid((p.rows + per_block - 1) / per_block), block(threads, per_block);
     auto scaled = [&]<int C, Scales S>() {
         auto kernel = p.residual ? norm_kernel<T, V, C, S, true, SHIFTED> : norm_kernel<T, V, C, S, false, SHIFTED>;
@@ -398,93 +431,135 @@ struct NormGradParams {
     bool weight_f32;
 };
 
-// Block b takes rows b, b + gridDim.x, ...; its share of dw stays in registers
-// (each thread keeps its columns) and goes out once.
-//
-// With whole vectors (V > 1) the rows pass through shared memory, kStages - 1
-// of them on their way while one is worked on: the registers hold dw and one
-// row, and could not hold another.  Each thread copies what it reads itself,
-// so a copy needs no barrier but the thread's own wait.
-constexpr int kMaxGradSmem = 2 * 3 * 16 * 4 * 512;
-template <int C> constexpr int kGradStages = C >= 4 ? 2 : 4;
+// Rows on their way through shared memory, kRowStages - 1 of them while one is
+// worked on, so that bytes in flight cost no registers.  Each thread copies
+// what it reads itself, so a copy needs no barrier but the thread's own wait.
+// A part of a chunk is copied as the whole 16 bytes that it lies in (a load
+// when it is read would hold up the block at every row) and masked when read.
+template <int C> constexpr int kRowStages = C >= 4 ? 2 : 4;
 
-template <typename T, int V, int C>
-__global__ void __launch_bounds__(512) norm_grad_kernel(const __grid_constant__ NormGradParams p) {
-    constexpr int kStages = kGradStages<C>;
-    using Vector = Pack<T, V>;
-    extern __shared__ __align__(16) unsigned char staged[];  // [kStages][3][C][threads] vectors
-    __shared__ float2 red[2][16];
-    const uint32_t t = threadIdx.x, step = blockDim.x * V;
-    const T *dy = static_cast<const T *>(p.dy), *x = static_cast<const T *>(p.x), *dsum = static_cast<const T *>(p.dsum);
-    auto slot = [&](uint32_t stage, int operand, int c) {
-        return reinterpret_cast<Vector *>(staged) + ((stage * 3 + operand) * C + c) * blockDim.x + t;
-    };
-    auto request = [&](uint32_t row, uint32_t stage) {
-        if constexpr (V > 1) {
-            if (row < p.rows) {
+template <typename T, int V, int C, int OPERANDS, bool SHIFTED> struct RowRing {
+    static constexpr int kStages = kRowStages<C>;
+    const T *base[OPERANDS];  // null: absent
+    int64_t stride[OPERANDS];
+    uint32_t rows;
+    const Chunks<V, C, SHIFTED> &chunks;
+    Pack<T, V> *slots;  // [kStages][OPERANDS][C][threads], 16 bytes each
+    uint32_t stage = 0;
+
+    __device__ RowRing(std::initializer_list<const void *> bases, std::initializer_list<int64_t> strides, uint32_t rows_,
+                       const Chunks<V, C, SHIFTED> &chunks_, void *smem)
+        : rows(rows_), chunks(chunks_), slots(static_cast<Pack<T, V> *>(smem)) {
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const uint32_t col = c * step + t * V;
-                    if (col >= p.cols) continue;
-                    copy16_async(slot(stage, 0, c), dy + row * p.dy_stride + col);
-                    copy16_async(slot(stage, 1, c), x + row * p.x_stride + col);
-                    if (dsum) copy16_async(slot(stage, 2, c), dsum + row * p.dsum_stride + col);
-                }
-            }
-            copies_commit();  // a group for every row, empty ones too
+        for (int o = 0; o < OPERANDS; ++o) {
+            base[o] = static_cast<const T *>(bases.begin()[o]);
+            stride[o] = strides.begin()[o];
         }
-    };
-    float dw[C][V];
-    Vector uw[C];
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const uint32_t col = c * step + t * V;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            dw[c][j] = 0.0f;
-            uw[c].e[j] = from_f32<T>(1.0f);
-        }
-        if (p.weight && !p.weight_f32 && col < p.cols)
-            uw[c] = *reinterpret_cast<const Vector *>(static_cast<const T *>(p.weight) + col);
+        for (int i = 0; i < kStages - 1; ++i) request(blockIdx.x + i * gridDim.x, i);
     }
-    // f32 weights beside 16-bit rows do not fit in uw: read again for each row, from L1.
-    auto weight = [&](int c, uint32_t col, float (&w)[V]) {
-        if (p.weight_f32) {
-            load_weight<T, V>(p.weight, true, col, w);
-        } else {
+    __device__ __forceinline__ Pack<T, V> *slot(uint32_t at, int operand, int c) const {
+        return slots + ((at * OPERANDS + operand) * C + c) * blockDim.x + threadIdx.x;
+    }
+    __device__ __forceinline__ void request(uint32_t row, uint32_t at) const {
+        if (row < rows) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) w[j] = to_f32(uw[c].e[j]);
-        }
-    };
+            for (int c = 0; c < C; ++c) {
+                const uint32_t col = chunks.first(c);
+                if (!chunks.some(c)) continue;
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) request(blockIdx.x + i * gridDim.x, i);
-    uint32_t turn = 0, stage = 0;
-    for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
-        Vector ug[C], ux[C];
-        if constexpr (V > 1) {
-            copies_wait<kStages - 2>();
-            // Into the slot that was read a row ago.
-            request(row + (kStages - 1) * gridDim.x, stage == 0 ? kStages - 1 : stage - 1);
+                for (int o = 0; o < OPERANDS; ++o)
+                    if (base[o]) copy16_async(slot(at, o, c), base[o] + row * stride[o] + (int32_t)col);
+            }
         }
-        float ss = 0.0f, gs = 0.0f;
+        copies_commit();  // a group for every row, empty ones too
+    }
+    // The row's copies are there; a later row's go to the slot read before.
+    __device__ __forceinline__ void next(uint32_t row) const {
+        copies_wait<kStages - 2>();
+        request(row + (kStages - 1) * gridDim.x, stage == 0 ? kStages - 1 : stage - 1);
+    }
+    __device__ __forceinline__ Pack<T, V> get(int operand, int c) const {
+        Pack<T, V> u = *slot(stage, operand, c);
+        if (SHIFTED && !chunks.whole(c)) {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (!chunks.has(chunks.first(c), j)) u.e[j] = from_f32<T>(0.0f);
+        }
+        return u;
+    }
+    __device__ __forceinline__ void done() { stage = stage + 1 == kStages ? 0 : stage + 1; }
+};
+
+// The thread's weights for the same columns of every row: in registers, but
+// f32 ones beside 16-bit rows, which do not fit there and are read again from L1.
+template <typename T, int V, int C, bool SHIFTED> struct RowWeights {
+    const void *weight;
+    bool again;
+    const Chunks<V, C, SHIFTED> &chunks;
+    Pack<T, V> kept[C];
+    __device__ RowWeights(const void *weight_, bool f32, const Chunks<V, C, SHIFTED> &chunks_)
+        : weight(weight_), again(weight_ && f32), chunks(chunks_) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const uint32_t col = c * step + t * V;
-            if (col < p.cols) {
-                if constexpr (V > 1) {
-                    ug[c] = *slot(stage, 0, c);
-                    ux[c] = *slot(stage, 1, c);
-                } else {
-                    ug[c].e[0] = dy[row * p.dy_stride + col];
-                    ux[c].e[0] = x[row * p.x_stride + col];
-                }
+            float w[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) w[j] = 1.0f;
+            if (!again && chunks.some(c)) chunks.template weights<T>(weight, false, c, w);
+#pragma unroll
+            for (int j = 0; j < V; ++j) kept[c].e[j] = from_f32<T>(w[j]);  // exact: they are of this type
+        }
+    }
+    __device__ __forceinline__ void get(int c, float (&w)[V]) const {
+        if (again) {
+            chunks.template weights<T>(weight, true, c, w);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) w[j] = to_f32(kept[c].e[j]);
+        }
+    }
+};
+
+// Block b takes rows b, b + gridDim.x, ... (SHIFTED: gridDim.x is a multiple of V
+// or covers the rows, so that all of a block's rows start the same distance
+// past a boundary); its share of dw stays in registers (each thread keeps its
+// columns) and goes out once.
+//
+// Measured at 8192 x 4096 bf16 with dsum: 104 us with rows loaded when they
+// are worked on, 51 us through the ring (5.3 TB/s) and 5 for the sum of the
+// blocks' dw; 8192 x 4095 105 us without dsum.  (The forward norm gains
+// nothing by a ring: 16384 x 4096 88 us against 90 without, narrow rows lose.)
+template <typename T, int V, int C, bool SHIFTED>
+__global__ void __launch_bounds__(512) norm_grad_kernel(const __grid_constant__ NormGradParams p) {
+    constexpr bool kHeld = C * V <= 16;  // the row's values stay in registers between their two uses
+    extern __shared__ __align__(16) unsigned char staged[];
+    __shared__ float2 red[2][16];
+    const Chunks<V, C, SHIFTED> chunks(p.cols, static_cast<const T *>(p.x) + blockIdx.x * p.x_stride, sizeof(T));
+    const RowWeights<T, V, C, SHIFTED> weights(p.weight, p.weight_f32, chunks);
+    RowRing<T, V, C, 3, SHIFTED> ring({p.x, p.dy, p.dsum}, {p.x_stride, p.dy_stride, p.dsum_stride}, p.rows, chunks, staged);
+    float dw[C][V];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < V; ++j) dw[c][j] = 0.0f;
+    uint32_t turn = 0;
+    for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+        ring.next(row);
+        float ss = 0.0f, gs = 0.0f;
+        Pack<T, V> ux[kHeld ? C : 1], ug[kHeld ? C : 1];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            if (chunks.some(c)) {
+                const int h = kHeld ? c : 0;
+                ux[h] = ring.get(0, c);
+                ug[h] = ring.get(1, c);
                 float w[V];
-                weight(c, col, w);
+                weights.get(c, w);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    const float s = to_f32(ux[c].e[j]);
+                    const float s = to_f32(ux[h].e[j]);
                     ss += s * s;
-                    gs += to_f32(ug[c].e[j]) * w[j] * s;
+                    gs += to_f32(ug[h].e[j]) * w[j] * s;
                 }
             }
         }
@@ -493,33 +568,43 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(const __grid_constant__ 
         const float back = rstd * rstd * rstd * (gs * p.per_col);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const uint32_t col = c * step + t * V;
-            if (col < p.cols) {
+            if (chunks.some(c)) {
+                const int h = kHeld ? c : 0;
+                if (!kHeld) {
+                    ux[0] = ring.get(0, c);
+                    ug[0] = ring.get(1, c);
+                }
                 float w[V], dx[V] = {};
-                if (dsum) {
-                    Vector u;
-                    if constexpr (V > 1) u = *slot(stage, 2, c);
-                    else u.e[0] = dsum[row * p.dsum_stride + col];
+                if (p.dsum) {
+                    const Pack<T, V> u = ring.get(2, c);
 #pragma unroll
                     for (int j = 0; j < V; ++j) dx[j] = to_f32(u.e[j]);
                 }
-                weight(c, col, w);
+                weights.get(c, w);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    const float s = to_f32(ux[c].e[j]), g = to_f32(ug[c].e[j]) * rstd;
+                    const float s = to_f32(ux[h].e[j]), g = to_f32(ug[h].e[j]) * rstd;
                     dw[c][j] += g * s;
                     dx[j] += g * w[j] - s * back;
                 }
-                store_as<T, V>(static_cast<T *>(p.dx) + (int64_t)row * p.cols + col, dx);
+                chunks.store(static_cast<T *>(p.dx) + (int64_t)row * p.cols, c, dx);
             }
         }
-        stage = stage + 1 == kStages ? 0 : stage + 1;
+        ring.done();
     }
     if (!p.partials) return;
+    float *mine = p.partials + (int64_t)blockIdx.x * p.cols;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        const uint32_t col = c * step + t * V;
-        if (col < p.cols) store_as<float, V>(p.partials + (int64_t)blockIdx.x * p.cols + col, dw[c]);
+        const uint32_t col = chunks.first(c);
+        if (!chunks.some(c)) continue;
+        if constexpr (!SHIFTED) {
+            store_as<float, V>(mine + col, dw[c]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (chunks.has(col, j)) mine[col + j] = dw[c][j];
+        }
     }
 }
 
@@ -584,36 +669,39 @@ template <typename W> __global__ void __launch_bounds__(1024) norm_dweight_kerne
     if (lane == 0 && mine < cols) dweight[mine] = from_f32<W>(sum);
 }
 
-template <typename T, int V>
+constexpr uint32_t kMaxRingSmem = 220 * 1024;  // of a block, and of an SM's blocks
+// Blocks an SM of the gradient's kernel: about 24 warps, as many as its
+// registers and its ring let run at once.  A narrow row has few of them.
+uint32_t grad_blocks_per_sm(uint32_t threads, size_t smem) {
+    return std::clamp(std::min(768 / threads, kMaxRingSmem / (uint32_t)smem), 1u, 4u);
+}
+
+template <typename T, int V, bool SHIFTED>
 heph_status launch_norm_grad(const NormGradParams &p, uint32_t partials, int sm_count, uint32_t *out_blocks, cudaStream_t stream) {
-    constexpr int kMost = 16 / V;  // chunks of a thread: 16 registers for each of five vectors
-    const uint32_t units = p.cols / V;
+    constexpr int kMost = 32 / V;  // chunks of a thread: 32 registers of dw
+    const uint32_t units = SHIFTED ? (p.cols + 2 * V - 2) / V : p.cols / V;
     uint32_t c = 1;
-    while (c < kMost && (units + c - 1) / c > 256) c *= 2;
+    while (c < kMost && (units + c - 1) / c > (c * V >= 16 ? 512 : 256)) c *= 2;
     const uint32_t threads = ((units + c - 1) / c + 31) / 32 * 32;
-    // As many blocks as run at once: two an SM of up to 256 threads, else one.
-    const uint32_t blocks = *out_blocks = threads <= 256 ? partials : std::min<uint32_t>(partials, sm_count);
-    if (threads > 512)
-        return launch_rows("long row norm gradient", norm_grad_long_kernel<T, V>, dim3(blocks), dim3(1024), 0, stream, p);
-    auto go = [&]<int C>() -> heph_status {
-        const size_t smem = V > 1 ? kGradStages<C> * 3 * 16 * C * threads : 0;
-        if (smem)
-            HEPH_CUDA_TRY(cudaFuncSetAttribute(norm_grad_kernel<T, V, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxGradSmem),
-                          HEPH_DISPATCH_FAILED, "row norm gradient shared memory");
-        return launch_rows("row norm gradient", norm_grad_kernel<T, V, C>, dim3(blocks), dim3(threads), smem, stream, p);
-    };
-    switch (c) {
-        case 1: return go.template operator()<1>();
-        case 2: return go.template operator()<2>();
-        case 4:
-            if constexpr (kMost >= 4) return go.template operator()<4>();
-            break;
-        case 8:
-            if constexpr (kMost >= 8) return go.template operator()<8>();
-            break;
-        default:
-            if constexpr (kMost >= 16) return go.template operator()<16>();
+    const size_t smem = (size_t)(c >= 4 ? kRowStages<4> : kRowStages<1>) * 3 * 16 * c * threads;
+    if (threads > 512 || smem > kMaxRingSmem) {
+        *out_blocks = std::min<uint32_t>(partials, sm_count);
+        if constexpr (!SHIFTED)
+            return launch_rows("long row norm gradient", norm_grad_long_kernel<T, V>, dim3(*out_blocks), dim3(1024), 0, stream, p);
+        return launch_rows("long row norm gradient", norm_grad_long_kernel<T, 1>, dim3(*out_blocks), dim3(1024), 0, stream, p);
     }
+    auto go = [&]<int C>() -> heph_status {
+        auto kernel = norm_grad_kernel<T, V, C, SHIFTED>;
+        const uint32_t step = SHIFTED ? V : 1, most = grad_blocks_per_sm(threads, smem) * sm_count / step * step;
+        *out_blocks = std::min(partials, most);
+        HEPH_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxRingSmem),
+                      HEPH_DISPATCH_FAILED, "row norm gradient shared memory");
+        return launch_rows("row norm gradient", kernel, dim3(*out_blocks), dim3(threads), smem, stream, p);
+    };
+    if (c == 1) return go.template operator()<1>();
+    if (c == 2) return go.template operator()<2>();
+    if (c == 4) return go.template operator()<4>();
+    if constexpr (kMost >= 8) return go.template operator()<8>();
     return fail(HEPH_DISPATCH_FAILED, "no row norm gradient kernel for this width");
 }
 
@@ -645,10 +733,15 @@ heph_status launch_rms_norm(const NormArgs &a, cudaStream_t stream) {
     });
 }
 
-uint32_t norm_grad_partials(uint32_t rows, int sm_count) { return std::min<uint32_t>(rows, 2 * sm_count); }
+// The most blocks that launch_norm_grad starts (4 an SM for rows of up to 192
+// threads, else 3), in whole vectors' worth.
+uint32_t norm_grad_partials(uint32_t rows, uint32_t cols, int sm_count) {
+    const uint32_t most = (cols <= 3000 ? 4 : 3) * (uint32_t)sm_count;
+    return rows < most ? rows : most / 8 * 8;
+}
 
 heph_status launch_rms_norm_backward(const NormGradArgs &a, int sm_count, cudaStream_t stream) {
-    const uint32_t partials = norm_grad_partials(a.rows, sm_count);
+    const uint32_t partials = norm_grad_partials(a.rows, a.cols, sm_count);
     uint32_t blocks = 0;  // of these used
     const NormGradParams p{a.dy.ptr, a.x.ptr, a.dsum.ptr, a.weight, a.dx, a.dweight ? a.partials : nullptr, a.dy.stride,
                            a.x.stride, a.dsum.stride, a.eps, 1.0f / a.cols, a.rows, a.cols, a.weight_f32};
@@ -657,8 +750,21 @@ heph_status launch_rms_norm_backward(const NormGradArgs &a, int sm_count, cudaSt
         if (a.rows) {
             const bool wide = a.cols % V == 0 && aligned_rows(a.dy, sizeof(T)) && aligned_rows(a.x, sizeof(T)) &&
                               aligned_rows(a.dsum, sizeof(T)) && aligned16(a.weight) && aligned16(a.dx);
-            const heph_status st = wide ? launch_norm_grad<T, V>(p, partials, sm_count, &blocks, stream)
-                                        : launch_norm_grad<T, 1>(p, partials, sm_count, &blocks, stream);
+            // Shifted rows, as in launch_rms_norm; else element by element.
+            auto like = [&](const void *ptr, int64_t stride) {
+                const auto apart = reinterpret_cast<intptr_t>(ptr) - reinterpret_cast<intptr_t>(a.x.ptr);
+                return !ptr || (apart % 16 == 0 && (stride - a.x.stride) % V == 0);
+            };
+            const bool shifted = like(a.dy.ptr, a.dy.stride) && like(a.dsum.ptr, a.dsum.stride) && like(a.dx, a.cols);
+            heph_status st;
+            if (wide) {
+                st = launch_norm_grad<T, V, false>(p, partials, sm_count, &blocks, stream);
+            } else if (shifted) {
+                st = launch_norm_grad<T, V, true>(p, partials, sm_count, &blocks, stream);
+            } else {
+                blocks = std::min<uint32_t>(partials, sm_count);
+                st = launch_rows("row norm gradient", norm_grad_long_kernel<T, 1>, dim3(blocks), dim3(1024), 0, stream, p);
+            }
             if (st != HEPH_OK) return st;
         }
         if (!a.dweight) return HEPH_OK;

@@ -44,9 +44,9 @@ struct NormGradArgs {
     uint32_t rows, cols;
     void *dx;
     void *dweight;      // of the weight's type; null with it
-    float *partials;    // norm_grad_partials(rows) x cols
+    float *partials;    // norm_grad_partials() x cols
 };
-uint32_t norm_grad_partials(uint32_t rows, int sm_count);
+uint32_t norm_grad_partials(uint32_t rows, uint32_t cols, int sm_count);
 heph_status launch_rms_norm_backward(const NormGradArgs &a, int sm_count, cudaStream_t stream);
 
 struct RouteArgs {
