@@ -124,22 +124,23 @@ __device__ __forceinline__ float scale_of(float amax) { return fmaxf(amax, kFp8F
 // ends, which are parts of chunks, are taken element by element.
 template <int V, int C, bool SHIFTED> struct Chunks {
     uint32_t cols, step, origin;
-    uint32_t wholes = 0, somes = 0;  // chunks that lie in the row, and of which some column does, a bit each
+    uint32_t wholes = 0, somes = 0;  // SHIFTED chunks that lie in the row, and of which some column does, a bit each
     __device__ Chunks(uint32_t cols_, const void *row, size_t size)
         : cols(cols_), step(blockDim.x * V),
           origin(threadIdx.x * V - (SHIFTED ? (uint32_t)((reinterpret_cast<uintptr_t>(row) & 15u) / size) : 0)) {
+        if (!SHIFTED) return;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const uint32_t col = first(c);
-            wholes |= (col < cols && (!SHIFTED || col + V <= cols) ? 1u : 0u) << c;
-            somes |= (SHIFTED ? col + V - 1 < cols + V - 1 : col < cols ? 1u : 0u) << c;
+            wholes |= (col < cols && col + V <= cols ? 1u : 0u) << c;
+            somes |= (col + V - 1 < cols + V - 1 ? 1u : 0u) << c;
         }
     }
     // Chunk c's first column; a SHIFTED row's first chunk starts before column
     // 0, and the number wraps.
     __device__ __forceinline__ uint32_t first(int c) const { return c * step + origin; }
-    __device__ __forceinline__ bool whole(int c) const { return wholes >> c & 1u; }
-    __device__ __forceinline__ bool some(int c) const { return somes >> c & 1u; }
+    __device__ __forceinline__ bool whole(int c) const { return SHIFTED ? wholes >> c & 1u : first(c) < cols; }
+    __device__ __forceinline__ bool some(int c) const { return SHIFTED ? somes >> c & 1u : first(c) < cols; }
     __device__ __forceinline__ bool has(uint32_t col, int j) const { return !SHIFTED || col + j < cols; }
 
     template <typename T> __device__ __forceinline__ Pack<T, V> load(const T *row, int c) const {
@@ -235,9 +236,14 @@ __device__ __forceinline__ void finish_row(const NormParams &p, uint32_t row, co
 }
 
 // A row (or, blockDim.y > 1, a row per warp) whose C x V values per thread
-// stay in registers between the one read and the one write.
+// stay in registers between the one read and the one write.  Bound by HBM,
+// and by the bytes in flight that fill it: rows wait for their sums, others
+// load meanwhile, so blocks an SM count.  16384 x 4096 bf16 with residual and
+// e4m3 scales by 128: four blocks (51 registers) 90 us, five 82.5 us (5.7
+// TB/s), six spill, 88 us; 5003 x 2049 f16 six blocks 16.4 us, five 17.4.
 template <typename T, int V, int C, Scales S, bool RES, bool SHIFTED>
-__global__ void __launch_bounds__(C * V >= 32 ? 512 : 1024) norm_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(C * V >= 32 ? 512 : 256, C * V >= 32 ? 1 : SHIFTED && S == kNoScales ? 6 : 5)
+norm_kernel(const __grid_constant__ NormParams p) {
     extern __shared__ float group_max[];  // kSharedScales: of each group
     __shared__ float2 red[32];
     const bool warp_rows = blockDim.y > 1;
