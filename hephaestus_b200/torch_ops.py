@@ -55,7 +55,9 @@ def _view(t: torch.Tensor) -> StridedView:
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """torch's current stream.  Its default stream is the legacy one, whose own
+    handle (cudaStreamLegacy) is passed: a null stream means the device's."""
+    return torch.cuda.current_stream().cuda_stream or 1
 
 
 def _full(op_code: int, t: torch.Tensor) -> torch.Tensor:
