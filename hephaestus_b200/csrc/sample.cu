@@ -220,7 +220,7 @@ __constant__ double kExp2[6] = {0x1.0000000000000p+0,  0x1.62e42fefa39f3p-5,  0x
 
 struct Weigher {
     float max, floor;  // floor: a lower logit has no mass
-    float top, slope32;  // max, or the largest finite number; slope in 32 bits
+    float top, slope32;  // max, or the largest finite number; twice the slope in 32 bits
     double slope;        // 16 log2(e) / T
     int scale_bits, limb_bits;
     const double *roots;  // kRoots in shared memory
@@ -229,7 +229,7 @@ struct Weigher {
         : max(max_), scale_bits(scale_bits_), limb_bits(limb_bits_), roots(roots_) {
         top = fminf(max, FLT_MAX);
         slope = 16 * 1.4426950408889634 / t;
-        slope32 = (float)slope;
+        slope32 = (float)(2.0 * slope);
         // Below half a unit; and no -inf, whatever the temperature.
         floor = fmaxf(__double2float_rd((double)max - (scale_bits + 1.5) * 0.6931471805599453 * t), -FLT_MAX);
     }
@@ -237,8 +237,9 @@ struct Weigher {
     // a unit is at least 2^-45 of the maximum's mass, which is 2^scale_bits.
     __device__ __forceinline__ uint64_t mass(float l) const {
         l = fminf(l, FLT_MAX);  // an infinity is equal to itself
-        // n = 16 log2(w) rounded, in the low bits of `at`.
-        const float magic = 0x1.8p23f, at = (l - top) * slope32 + magic;
+        // n = 16 log2(w) rounded, in the low bits of `at`.  From halves, as l -
+        // top may pass the largest number.
+        const float magic = 0x1.8p23f, at = fmaf(l, 0.5f, -0.5f * top) * slope32 + magic;
         const uint32_t n = __float_as_uint(at);
         const double r = fma((double)l - (double)top, slope, -(double)(at - magic));
         double p = kExp2[5];

@@ -476,7 +476,9 @@ heph_status heph_reduce_full_noalloc(heph_op op, heph_dtype in_dtype, heph_dtype
 
 /* No counterparts in the reference.  Operators over the rows of a matrix in
  * caller-owned device memory of device `ordinal`: columns are adjacent, row r
- * starts `stride` elements after row r-1 (0 repeats a row).  They allocate
+ * starts `stride` elements after row r-1 (0 repeats a row).  Rows may start on
+ * any element; the 16 bytes, from boundary to boundary, that hold a row's
+ * first or last element may be read whole, never written.  They allocate
  * nothing and need no heph_device; a NULL stream is the legacy default
  * stream; the calling thread's current device is left as it was.  Outputs are
  * contiguous and must not alias an input or one another.  Calls may run at

@@ -483,6 +483,18 @@ def test_sample_tiny_temperatures(T):
     assert tokens.tolist() == [100, 100, 4000, 4000]
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sample_logits_over_the_whole_range(T, dtype):
+    """The largest minus the least passes the largest number of 32 bits."""
+    g = torch.Generator(device="cuda").manual_seed(12)
+    logits = ((torch.rand(5, 6000, device="cuda", generator=g) * 2 - 1) * 3.38e38).to(dtype)
+    logits[0, 7], logits[1, 9] = torch.finfo(dtype).max, torch.finfo(dtype).min
+    u = torch.rand(5, device="cuda", generator=g)
+    for t in (1.0, 1e36, 1e38, 3e38, 1e300):
+        for kw in (dict(), dict(top_p=0.6), dict(top_k=50), dict(top_k=4000, top_p=0.7)):
+            check_sample(T, logits, u, temperature=t, **kw)
+
+
 def test_sample_numbers_outside_the_range(T):
     logits = rand(4, 1000, seed=1)
     u = torch.tensor([-1.0, 1.0, float("nan"), 2.0], device="cuda")
@@ -590,6 +602,76 @@ def test_trains_through_an_autograd_function(T):
     near(x.grad, want, size, 2 * FOLD)
     assert torch.equal(x.grad, r.grad)
     near(w.grad, want_w, size_w, 2 * FOLD)
+
+
+def test_calls_from_several_threads(T):
+    """Each thread on a stream of its own, all operators, the answers of one thread alone."""
+    import threading
+    x, w = rand(500, 1000, dtype=torch.bfloat16, seed=1), rand(1000, seed=2)
+    logits = rand(300, 160, seed=3)
+    vocab = rand(30, 40000, seed=4, scale=2)
+    u = torch.rand(30, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5))
+    pairs = torch.randint(0, 160, (100000,), device="cuda", dtype=torch.int32)
+
+    def work():
+        ds, dw = T.rms_norm_backward(x, x, w)
+        q, scale = T.rms_norm_fp8(x, w, group=64)
+        weights, picks = T.route_experts(logits, 6, score="sigmoid", groups=8, groups_kept=4)
+        return [T.rms_norm(x, w), ds, dw, q.view(torch.uint8), scale, weights, picks,
+                T.route_experts_backward(weights, logits, picks, score="sigmoid"), *T.expert_order(picks, 160),
+                *T.expert_order(pairs, 160), *T.sample_tokens(vocab, u, top_k=50, top_p=0.9), *T.sample_tokens(vocab, u)]
+
+    want = work()
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run():
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    got = work()
+                    stream.synchronize()
+                    wrong.extend(i for i, (a, b) in enumerate(zip(got, want)) if not torch.equal(a, b))
+        except Exception as e:  # a thread's own is lost
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=run) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_rows_more_than_32_bits_apart(T):
+    """Inputs and outputs past 2^31 elements: the last rows are the right ones."""
+    apart = 2 ** 31 + 64
+    base = torch.empty(apart + 9000, device="cuda", dtype=torch.bfloat16)
+    near_rows = rand(2, 9000, dtype=torch.bfloat16, seed=1, scale=2)
+    x = base.as_strided((2, 9000), (apart, 1))
+    x.copy_(near_rows)
+    u = torch.tensor([0.2, 0.8], device="cuda")
+    for cols in (4096, 4095, 9000):
+        a, b = x[:, :cols], near_rows[:, :cols]
+        for got, want in zip((T.rms_norm(a), *T.rms_norm_fp8(a, group=128)), (T.rms_norm(b), *T.rms_norm_fp8(b, group=128))):
+            assert torch.equal(got.float(), want.float())
+        assert torch.equal(T.rms_norm_backward(a, a)[0], T.rms_norm_backward(b, b)[0])
+        for kw in (dict(), dict(top_k=9), dict(top_p=0.5)):
+            assert torch.equal(T.sample_tokens(a, u, **kw)[0], T.sample_tokens(b, u, **kw)[0])
+    a, b = x[:, :200], near_rows[:, :200]
+    picked, want = T.route_experts(a, 8), T.route_experts(b, 8)
+    assert torch.equal(picked[0], want[0]) and torch.equal(picked[1], want[1])
+    assert torch.equal(T.route_experts_backward(want[0], a, want[1]), T.route_experts_backward(want[0], b, want[1]))
+    del x, base
+    rows = 2 ** 19 + 3  # of 4096: outputs past 2^31 elements
+    tall = near_rows[:1, :4096].expand(rows, 4096)
+    w = rand(4096, seed=2)
+    y = T.rms_norm(tall, w)
+    ds, dw = T.rms_norm_backward(tall, tall, w)
+    one = T.rms_norm(tall[:1], w), T.rms_norm_backward(tall[:1], tall[:1], w)[0]
+    for i in (0, 2 ** 19 - 1, 2 ** 19, rows - 1):
+        assert torch.equal(y[i:i + 1], one[0]) and torch.equal(ds[i:i + 1], one[1])
 
 
 def test_leaves_its_surroundings_alone(T):
