@@ -64,13 +64,15 @@ def _compile(src: str, verbose_ptxas: bool) -> str:
     return obj
 
 
-def build_torch_module(force: bool = False) -> str:
-    """``_torch_rows.so``: the torch boundary of the row operators, beside LIB."""
+def build_torch_module(force: bool = False) -> str | None:
+    """``_torch_rows.so``: the torch boundary of the row operators, beside LIB.
+
+    None, and no module, without a CUDA build of torch: LIB does not need one."""
     src = os.path.join(CSRC, "torch_rows.cpp")
     spec = importlib.util.find_spec("torch")
-    if spec is None:
-        raise RuntimeError("torch is needed to build _torch_rows.so")
-    torch_dir = os.path.dirname(spec.origin)
+    torch_dir = os.path.dirname(spec.origin) if spec else ""
+    if not os.path.exists(os.path.join(torch_dir, "include", "c10", "cuda", "CUDAStream.h")):
+        return None
     newest_dep = max(os.path.getmtime(p) for p in [src, __file__, spec.origin] + headers())
     if os.path.exists(TORCH_MODULE) and os.path.getmtime(TORCH_MODULE) >= newest_dep and not force:
         return TORCH_MODULE

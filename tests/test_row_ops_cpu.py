@@ -183,6 +183,12 @@ def test_c_sample_refusals():
         c_refused(message, "heph_sample_tokens", *args(**kw))
 
 
+def test_the_library_builds_without_torch(monkeypatch):
+    from hephaestus_b200 import build
+    monkeypatch.setattr(build.importlib.util, "find_spec", lambda name: None)
+    assert build.build_torch_module() is None
+
+
 def test_an_empty_call_needs_no_device():
     """Nothing to do is done without touching a device (none is here in the CPU suite)."""
     assert N.lib.heph_rms_norm(*norm_args(rows=0, x=None, y=None)) == N.OK
