@@ -52,8 +52,9 @@ struct SampleParams {
     const int32_t *top_k;
     double temperature_all, top_p_all, min_p_all;
     int32_t top_k_all;
-    uint32_t vocab;
+    uint32_t rows, vocab;
     int scale_bits, limb_bits;
+    bool deal;  // rows of long work first
     int64_t *tokens;
     float *probs;
 };
@@ -85,6 +86,7 @@ struct SampleShared {
     double roots[16];
     uint32_t listed[2];  // entries in `list`, and in `mass` where that is the second list
     Threshold keep;
+    uint32_t row;  // that is worked on
     uint32_t found_bin;
     uint64_t found_above, found_in;
 };
@@ -576,21 +578,59 @@ __device__ void draw_from_list(const T *row, const Weigher &weigh, SampleShared 
     }
 }
 
+// What a row asks for.
+struct Asked {
+    double t, top_p;
+    int32_t k;
+    bool greedy, by_count, by_mass;
+    __device__ Asked(const SampleParams &p, uint32_t row)
+        : t(p.temperature ? p.temperature[row] : p.temperature_all), top_p(p.top_p ? p.top_p[row] : p.top_p_all),
+          k(p.top_k ? p.top_k[row] : p.top_k_all) {
+        greedy = !(t > 0.0) || k == 1;
+        by_count = !greedy && k > 0 && (uint32_t)k < p.vocab;
+        by_mass = !greedy && top_p < 1.0;
+    }
+    // Most work first.
+    __device__ __forceinline__ uint32_t order() const { return by_mass && !by_count ? 0 : greedy ? 2 : 1; }
+};
+
+// The row that is `place`-th by order(), then by index; of at most
+// kSampleThreads rows, a thread each.
+__device__ uint32_t dealt_row(const SampleParams &p, SampleShared &s, uint32_t place) {
+    const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const uint32_t order = t < p.rows ? Asked(p, t).order() : 3;
+    const uint32_t first = __syncthreads_count(order == 0), second = __syncthreads_count(order == 1);
+    const uint32_t alike = __match_any_sync(kFullMask, order);
+    // Rows of each order in the warps below, ten bits each.
+    if (lane == 0) s.scan[warp] = 0;
+    __syncwarp();
+    if (order < 3 && lane == __ffs(alike) - 1u) atomicAdd((unsigned long long *)&s.scan[warp], (unsigned long long)__popc(alike) << order * 10);
+    __syncthreads();
+    uint64_t below = 0;
+#pragma unroll
+    for (int w = 0; w < kSampleWarps; ++w) below += w < (int)warp ? s.scan[w] : 0;
+    const uint32_t at = (order > 0 ? first : 0) + (order > 1 ? second : 0) + (uint32_t)(below >> (order * 10) & 1023u) +
+                        __popc(alike & ((1u << lane) - 1));
+    if (order < 3 && at == place) s.row = t;
+    __syncthreads();
+    return s.row;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_constant__ SampleParams p) {
     __shared__ SampleShared s;
     const cg::cluster_group cluster = cg::this_cluster();
     const uint32_t blocks = cluster.num_blocks(), block = cluster.block_rank();
-    const uint32_t row = blockIdx.x / blocks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t row = p.deal ? dealt_row(p, s, blockIdx.x / blocks) : blockIdx.x / blocks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const RowPart<T> part(static_cast<const T *>(p.logits) + row * p.stride, p.vocab, blocks * kSampleWarps,
                           block * kSampleWarps + warp);
-    double t = p.temperature ? p.temperature[row] : p.temperature_all;
-    const int32_t k = p.top_k ? p.top_k[row] : p.top_k_all;
-    const double top_p = p.top_p ? p.top_p[row] : p.top_p_all;
+    const Asked asked(p, row);
+    double t = asked.t;
+    const int32_t k = asked.k;
+    const double top_p = asked.top_p;
     const double min_p = p.min_p ? p.min_p[row] : p.min_p_all;
     const float u = p.uniform[row];
-    const bool greedy = !(t > 0.0) || k == 1;
-    const bool by_count = !greedy && k > 0 && (uint32_t)k < p.vocab, by_mass = !greedy && top_p < 1.0;
+    const bool greedy = asked.greedy, by_count = asked.by_count, by_mass = asked.by_mass;
 
     // The maximum, and for top-k the mean, which tells the logits' scale.
     float max = -INFINITY, sum = 0.0f;
@@ -875,18 +915,25 @@ heph_status launch_sample(const SampleArgs &a, int sm_count, cudaStream_t stream
     // much in theirs, never over a share of 64 K logits each.  Measured on one
     // B200 with 1 / 2 / 4 / 8 blocks a row: 1 row of 131072 41 / 29 / 22 / 21
     // us, 128 of 50257 27 / 31 / 43 / 65, 256 of 131072, each with settings of
-    // its own, 233 / 173 / 167 / 226.
+    // its own and in the order of their index, 233 / 173 / 167 / 226.
     uint32_t blocks = 1;
     while (blocks < kMaxCluster && (((uint64_t)a.rows * blocks * 2 <= (uint32_t)sm_count && a.vocab / (blocks * 2) >= 4096) ||
                                     a.vocab / blocks >= 65536))
         blocks *= 2;
+    // Rows that differ in their work and do not all run at once: the longest
+    // start first, or they end alone.  Top-p rows take 3 to 5 times as long as
+    // greedy ones: 256 of 131072 take 163 us in the order of their index, 150 in that of
+    // their work.  Each block finds its row itself, from the settings (where all
+    // are alike, 118 us instead of 115).
+    const bool deal = (a.temperature || a.top_p || a.top_k) && (uint64_t)a.rows * blocks > 2 * (uint32_t)sm_count &&
+                      a.rows <= kSampleThreads;
     // vocab x 2^scale_bits stays below 2^62, a mass below that of three limbs,
     // and the sum of a limb of a block's logits (an eighth of the row and 4096,
     // or less than 2^17) below 2^32.
     const int bits = 32 - __builtin_clz(a.vocab), limb_bits = a.vocab <= (1u << 20) - (1u << 16) ? 15 : 13;
     const SampleParams p{a.logits.ptr, a.logits.stride, a.uniform, a.temperature, a.top_p, a.min_p, a.top_k,
-                         a.temperature_all, a.top_p_all, a.min_p_all, a.top_k_all, a.vocab, std::min(3 * limb_bits - 1, 62 - bits), limb_bits,
-                         a.tokens, a.probs};
+                         a.temperature_all, a.top_p_all, a.min_p_all, a.top_k_all, a.rows, a.vocab,
+                         std::min(3 * limb_bits - 1, 62 - bits), limb_bits, deal, a.tokens, a.probs};
     return dispatch_row_dtype(a.dtype, [&]<typename T>() -> heph_status {
         return launch_clusters("token sampling", sample_kernel<T>, dim3(a.rows * blocks), dim3(kSampleThreads), blocks, 0,
                                stream, p);

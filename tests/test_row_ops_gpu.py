@@ -415,6 +415,26 @@ def test_sample_is_the_same_in_any_batch(T):
             assert torch.equal(part[0], whole[0][:n]) and torch.equal(part[1], whole[1][:n])
 
 
+@pytest.mark.parametrize("rows", [296, 297, 320, 511, 512, 513])
+def test_sample_rows_in_the_order_of_their_work(T, rows):
+    """Batches whose long rows start first: each row's answer is that of a small batch."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    logits = rand(rows, 2500, seed=rows, scale=2.5)
+    u = torch.rand(rows, device="cuda", generator=g)
+    t = torch.rand(rows, device="cuda", generator=g) * 1.5
+    t[torch.rand(rows, device="cuda", generator=g) < 0.3] = 0.0
+    k = torch.randint(-60, 60, (rows,), device="cuda", dtype=torch.int32, generator=g)
+    p = torch.rand(rows, device="cuda", generator=g) * 1.5
+    alike = [torch.full_like(t, 0.0), torch.full_like(t, 0.8)]
+    for temperature in (t, *alike):
+        for top_k, top_p in ((k, p), (0, p), (k, 1.0), (0, 1.0)):
+            got = T.sample_tokens(logits, u, temperature=temperature, top_k=top_k, top_p=top_p)
+            for i in range(0, rows, 100):
+                part = [v[i:i + 100] if torch.is_tensor(v) else v for v in (temperature, top_k, top_p)]
+                want = T.sample_tokens(logits[i:i + 100], u[i:i + 100], temperature=part[0], top_k=part[1], top_p=part[2])
+                assert torch.equal(got[0][i:i + 100], want[0]) and torch.equal(got[1][i:i + 100], want[1])
+
+
 def test_sample_ties_and_masks(T):
     v = 5000
     u = torch.tensor([0.0, 0.2, 0.5, 0.75, 0.999999], device="cuda")
