@@ -197,6 +197,7 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) expert_order_k
 __host__ __device__ constexpr uint32_t counts_pitch(uint32_t experts) { return (experts + 3) / 4 * 4; }
 __global__ void __launch_bounds__(kMany) expert_count_kernel(const int32_t *picks, uint32_t count, uint32_t experts, uint32_t *counts) {
     extern __shared__ uint32_t smem[];
+    let_next_start();
     using Part = OrderPart<kMany>;
     const Part part(picks, count, experts, gridDim.x, blockIdx.x, smem);
     uint32_t total[Part::kExpertsPerThread];
@@ -216,6 +217,7 @@ __global__ void __launch_bounds__(kMany) expert_place_kernel(const int32_t *pick
     const Part part(picks, count, experts, gridDim.x, blockIdx.x, smem);
     uint32_t before[Part::kExpertsPerThread] = {}, all[Part::kExpertsPerThread];
     part.count(all);
+    after_previous();  // its own counts need nothing of the first launch
     const uint32_t pitch = counts_pitch(experts), quads = pitch / 4, rows = kMany / quads;
     const uint32_t quad = threadIdx.x % quads, first = threadIdx.x / quads;
     if (first < rows) {
@@ -270,7 +272,8 @@ size_t expert_order_workspace(uint32_t count, uint32_t experts) {
 heph_status launch_expert_order(const int32_t *picks, uint32_t count, uint32_t experts, int32_t *offsets,
                                 int32_t *order, int32_t *slot, uint32_t *workspace, cudaStream_t stream) {
     // Measured for 64 x 8 / 32768 x 8 pairs of 256 experts: 5.4 / 16.4 us with
-    // blocks of 256 threads throughout, 5.8 / 14.3 us with these.
+    // blocks of 256 threads throughout, 5.8 / 14.3 us with these, and 11.6 with
+    // the second launch's own counts during the first.
     if (count <= 2 * kSteps * kFew)
         return launch_clusters("expert order", expert_order_kernel<kFew>, dim3(1), dim3(kFew), 1, order_smem(kFew, experts), stream,
                                picks, count, experts, offsets, order, slot);
@@ -291,7 +294,7 @@ heph_status launch_expert_order(const int32_t *picks, uint32_t count, uint32_t e
     if ((st = allow_smem(expert_count_kernel)) != HEPH_OK || (st = allow_smem(expert_place_kernel)) != HEPH_OK) return st;
     st = launch_rows("expert counts", expert_count_kernel, grid, dim3(kMany), smem, stream, picks, count, experts, workspace);
     if (st != HEPH_OK) return st;
-    return launch_rows("expert order", expert_place_kernel, grid, dim3(kMany), smem, stream, picks, count, experts, workspace,
+    return launch_next("expert order", expert_place_kernel, grid, dim3(kMany), smem, stream, picks, count, experts, workspace,
                        offsets, order, slot);
 }
 

@@ -64,6 +64,28 @@ heph_status launch_rows(const char *what, void (*kernel)(P...), dim3 grid, dim3 
     return HEPH_OK;
 }
 
+// A kernel that follows another of the same call: its blocks may start before
+// that one ends, from its let_next_start() on, and see what it wrote after
+// after_previous().
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <typename... P, typename... A>
+heph_status launch_next(const char *what, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                        A &&...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    HEPH_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, P(args)...), HEPH_DISPATCH_FAILED, what);
+    return HEPH_OK;
+}
+
 // The same with the blocks in clusters of `cluster`.
 template <typename... P, typename... A>
 heph_status launch_clusters(const char *what, void (*kernel)(P...), dim3 grid, dim3 block, uint32_t cluster, size_t smem,

@@ -624,6 +624,51 @@ def test_trains_through_an_autograd_function(T):
     near(w.grad, want_w, size_w, 2 * FOLD)
 
 
+def test_calls_of_two_kernels_one_after_the_other(T):
+    """The second kernel of a call starts before the first ends: calls that write each other's
+    inputs, in a stream and in a graph, between reductions that start early too."""
+    picks = torch.randint(0, 60, (80000,), device="cuda", dtype=torch.int32,
+                          generator=torch.Generator(device="cuda").manual_seed(1))
+    x, w = rand(700, 1000, seed=2), rand(1000, seed=3)
+
+    def chain():
+        out, now, grad = [], picks, x
+        for _ in range(6):
+            offsets, order, slot = T.expert_order(now, 60)
+            total = T.sum(offsets)
+            now = (order + slot) % 60  # the next call's
+            grad, dw = T.rms_norm_backward(grad, x + grad, w)
+            out += [offsets, order, slot, total.clone(), grad, dw]
+        return out
+
+    want = []
+    now, grad = picks, x
+    for _ in range(6):
+        torch.cuda.synchronize()
+        offsets, order, slot = T.expert_order(now, 60)
+        torch.cuda.synchronize()
+        total = T.sum(offsets)
+        torch.cuda.synchronize()
+        now = (order + slot) % 60
+        torch.cuda.synchronize()
+        grad, dw = T.rms_norm_backward(grad, x + grad, w)
+        torch.cuda.synchronize()
+        want += [offsets, order, slot, total, grad, dw]
+    for _ in range(3):
+        for a, b in zip(chain(), want):
+            assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        offsets, order, slot = T.expert_order(picks, 60)
+        again = T.expert_order((order + slot) % 60, 60)
+        ds, dw = T.rms_norm_backward(x, x + x, w)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip((offsets, order, slot, *again, ds, dw), (*want[:3], *want[6:9], *want[4:6])):
+        assert torch.equal(a, b)
+
+
 def test_calls_from_several_threads(T):
     """Each thread on a stream of its own, all operators, the answers of one thread alone."""
     import threading
