@@ -412,18 +412,21 @@ __device__ Narrowed narrow(const RowPart<T> &part, const Weigher &weigh, SampleS
         Histogram &h = s.hist[turn];
         turn ^= 1;
         clear(h);
-        // Logits that may be counted now; all others are passed over.
-        const float from = shift < 0 ? floor : key_value(low), upto = shift < 0 ? INFINITY : key_value(high);
+        // Logits that may be counted now; all others are passed over.  Whether a
+        // logit is between the keys is asked of its own key: 0x7fffffff is no
+        // number's (both zeros have 0x80000000), and as a float it is -0.
+        const float from = shift < 0 ? floor : key_value(low);
         part.each([&](const float(&v)[RowPart<T>::V], uint32_t) {
             if (!(largest(v) >= from)) return;
 #pragma unroll
             for (int j = 0; j < RowPart<T>::V; ++j) {
                 const float l = v[j];
-                if (!(l >= from && l <= upto && l > floor)) continue;
+                if (!(l >= from && l > floor)) continue;
                 uint32_t bin = steps.bin(l);
                 if (shift >= 0) {
-                    if (bin != first) continue;
-                    bin = (high - ordered_number(l)) >> shift;
+                    const uint32_t key = ordered_number(l);
+                    if (bin != first || key < low || key > high) continue;
+                    bin = (high - key) >> shift;
                 }
                 if constexpr (MASS) mass_to_bin(weigh, h, bin, l);
                 else atomicAdd(&h.limb[0][bin], 1u);
