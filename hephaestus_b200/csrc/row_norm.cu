@@ -55,11 +55,16 @@ __device__ __forceinline__ void load_weight(const void *weight, bool f32, uint32
     }
 }
 
+// Accesses of 16 bytes at most: what operands and the workspace are aligned to.
 template <typename T, int V> __device__ __forceinline__ void store_as(T *dst, const float (&v)[V]) {
-    Pack<T, V> u;
+    constexpr int N = V * sizeof(T) <= 16 ? V : 16 / sizeof(T);
 #pragma unroll
-    for (int j = 0; j < V; ++j) u.e[j] = from_f32<T>(v[j]);
-    *reinterpret_cast<Pack<T, V> *>(dst) = u;
+    for (int i = 0; i < V / N; ++i) {
+        Pack<T, N> u;
+#pragma unroll
+        for (int j = 0; j < N; ++j) u.e[j] = from_f32<T>(v[i * N + j]);
+        *reinterpret_cast<Pack<T, N> *>(dst + i * N) = u;
+    }
 }
 
 template <int V> __device__ __forceinline__ void store_fp8(void *dst, const float (&v)[V]) {

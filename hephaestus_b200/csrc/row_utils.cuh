@@ -18,8 +18,10 @@ template <typename T> __device__ __forceinline__ T from_f32(float v) {
     else return __float2half_rn(v);
 }
 
-// N adjacent elements, moved by one access.
+// N adjacent elements, moved by one access: of 16 bytes at most, as no operand
+// or workspace is known to be aligned to more.
 template <typename T, int N> struct alignas(sizeof(T) * N) Pack {
+    static_assert(sizeof(T) * N <= 16);
     T e[N];
 };
 

@@ -3,6 +3,8 @@ neighbouring numbers, NaN in biases, workspaces on the least alignment that is a
 
 Against the 64-bit forms, with the tolerances of test_row_ops_gpu.py.
 """
+import ctypes
+
 import pytest
 import torch
 
@@ -10,6 +12,32 @@ from tests import row_ops_ref as ref
 from tests.test_row_ops_gpu import FOLD, T, check_route, check_sample, near, rand  # noqa: F401  (T: the fixture)
 
 pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------- norm
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cols", [64, 1000, 4096, 40000])
+def test_rms_norm_backward_workspace_on_16_bytes(T, dtype, cols):
+    """The workspace is asked for on 16 bytes: one that is on no 32 will do."""
+    from hephaestus_b200 import _native as N
+    code = {torch.float32: N.ROW_F32, torch.bfloat16: N.ROW_BF16, torch.float16: N.ROW_F16}[dtype]
+    rows = 40
+    dy, s, w = rand(rows, cols, dtype=dtype, seed=1), rand(rows, cols, dtype=dtype, seed=2), rand(cols, dtype=dtype, seed=3)
+    dx, dw = torch.empty_like(s), torch.empty_like(w)
+    need = ctypes.c_uint64()
+    assert N.lib.heph_rms_norm_backward_workspace(0, rows, cols, ctypes.byref(need)) == N.OK
+    memory = torch.full((need.value + 96,), 0xa5, dtype=torch.uint8, device="cuda")
+    at = 16 + -memory.data_ptr() % 32  # 16 past a multiple of 32
+    torch.cuda.synchronize()
+    assert N.lib.heph_rms_norm_backward(0, code, dy.data_ptr(), cols, s.data_ptr(), cols, None, 0, w.data_ptr(), code, 1e-6, rows,
+                                        cols, dx.data_ptr(), dw.data_ptr(), memory.data_ptr() + at, need.value, None) == N.OK
+    torch.cuda.synchronize()
+    want, want_w, size, size_w = ref.rms_norm_grads(dy, s, w, 1e-6)
+    near(dx, want, size, 2 * FOLD)
+    near(dw, want_w, size_w, 2 * FOLD)
+    assert bool((memory[:at] == 0xa5).all()) and bool((memory[at + need.value:] == 0xa5).all())
 
 
 # --------------------------------------------------------------- sampling
