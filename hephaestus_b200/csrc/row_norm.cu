@@ -21,7 +21,9 @@ namespace heph {
 namespace {
 
 constexpr float kFp8Max = 448.0f;       // largest finite e4m3 value
-constexpr float kFp8Floor = 0x1p-100f;  // smallest maximum a scale is made for: keeps 1 / scale finite
+// Smallest maximum a scale is made for: keeps 1 / scale finite.  Its product
+// with rstd need not be, so values take rstd first and 1 / scale then.
+constexpr float kFp8Floor = 0x1p-100f;
 
 struct NormParams {
     const void *x, *residual, *weight;
@@ -194,10 +196,10 @@ __device__ __forceinline__ void finish_row(const NormParams &p, uint32_t row, co
     const float rstd = rsqrtf(ss * p.per_col + p.eps);
     // |w s| rstd rounds monotonically, so the maximum of |y| is the rounded
     // product of the maximum of |w s|.
-    float scale, factor = rstd;
+    float scale, per_scale = 1.0f;
     if (S == kRowScale) {
         scale = scale_of(amax * rstd);
-        factor = rstd * __fdividef(1.0f, scale);
+        per_scale = __fdividef(1.0f, scale);
         if (threadIdx.x == 0) p.scales[row] = scale;
     }
 #pragma unroll
@@ -207,7 +209,7 @@ __device__ __forceinline__ void finish_row(const NormParams &p, uint32_t row, co
         if (S == kLaneScales || (S == kSharedScales && !SHIFTED)) {
             const uint32_t g = col >> p.group_shift;
             scale = scale_of((S == kLaneScales ? gmax[c] : group_max[g]) * rstd);
-            factor = rstd * __fdividef(1.0f, scale);
+            per_scale = __fdividef(1.0f, scale);
             if (col == g << p.group_shift) p.scales[(int64_t)row * p.groups + g] = scale;
         }
         if (S == kSharedScales && SHIFTED) {
@@ -216,12 +218,12 @@ __device__ __forceinline__ void finish_row(const NormParams &p, uint32_t row, co
                 if (!chunks.has(col, j)) continue;
                 const uint32_t g = (col + j) >> p.group_shift;
                 scale = scale_of(group_max[g] * rstd);
-                v[c][j] *= rstd * __fdividef(1.0f, scale);
+                v[c][j] = v[c][j] * rstd * __fdividef(1.0f, scale);
                 if (col + j == g << p.group_shift) p.scales[(int64_t)row * p.groups + g] = scale;
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[c][j] *= factor;
+            for (int j = 0; j < V; ++j) v[c][j] = S == kNoScales ? v[c][j] * rstd : v[c][j] * rstd * per_scale;
         }
         if constexpr (S == kNoScales) {
             chunks.store(static_cast<T *>(p.y) + (int64_t)row * p.cols, c, v[c]);
@@ -369,9 +371,9 @@ template <typename T, int V, bool FP8> __global__ void __launch_bounds__(1024) n
         if constexpr (FP8) {
             const uint32_t g = by_group ? col >> p.group_shift : 0;
             const float scale = scale_of((by_group ? group_max[g] : amax) * rstd);
-            const float factor = rstd * __fdividef(1.0f, scale);
+            const float per_scale = __fdividef(1.0f, scale);
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] *= factor;
+            for (int j = 0; j < V; ++j) v[j] = v[j] * rstd * per_scale;
             store_fp8<V>(static_cast<uint8_t *>(p.y) + at, v);
             if (by_group ? col == g << p.group_shift : col == 0) p.scales[(int64_t)row * p.groups + g] = scale;
         } else {

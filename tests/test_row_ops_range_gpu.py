@@ -40,6 +40,49 @@ def test_rms_norm_backward_workspace_on_16_bytes(T, dtype, cols):
     assert bool((memory[:at] == 0xa5).all()) and bool((memory[at + need.value:] == 0xa5).all())
 
 
+# The kernels of e4m3 output: scales of groups of lanes, of groups past a warp's lanes, of the row, rows
+# of one warp, shifted rows (odd widths) with and without groups, long rows with and without.
+FP8_FORMS = [(64, None), (256, 16), (4096, None), (4096, 128), (4096, 1024), (2049, None), (2049, 128), (36864, None),
+             (36864, 128), (33001, None), (33001, 64)]
+
+
+def check_fp8(T, x, w, eps, group):
+    q, scale = T.rms_norm_fp8(x, w, eps, group=group)
+    want, _ = ref.rms_norm(x, w, eps)
+    near(scale, ref.scales(want, group))
+    cols = x.shape[1]
+    g = group if group and group < cols else cols
+    ratio = want / scale.double().repeat_interleave(g, dim=1)[:, :cols]
+    # Half a step of e4m3 (relative 2^-4, 2^-10 below its normal values), after the 32-bit value.
+    off = (q.double() - ratio).abs()
+    assert bool((off <= (2.0 ** -4 + 2 * FOLD) * ratio.abs() + 2.0 ** -10).all())
+    return q, scale
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cols,group", FP8_FORMS)
+def test_rms_norm_fp8_zeros_at_a_small_eps(T, dtype, cols, group):
+    """rstd / scale passes the largest number where the values are zeros: they stay zeros."""
+    x, w = rand(4, cols, dtype=dtype, seed=1), rand(cols, dtype=dtype, seed=2)
+    x[0] = 0
+    x[2, : cols // 2] = 0  # groups of zeros, or of zero weights, in rows that are not
+    x[3] = 0
+    x[3, cols - 1] = torch.finfo(dtype).smallest_normal if dtype == torch.float16 else 1e-7  # and in a row of tiny rms
+    w[cols // 4:cols // 2] = 0
+    for eps in (1e-12, 1e-30):
+        q, scale = check_fp8(T, x, w, eps, group)
+        assert bool((q[0].float() == 0).all()) and bool((q.float()[:, cols // 4:cols // 2] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cols,group", FP8_FORMS)
+def test_rms_norm_fp8_below_the_least_scale(T, dtype, cols, group):
+    """Values whose scale is the least one come out in its units."""
+    x, w = rand(3, cols, seed=3, scale=5e-38).to(dtype), rand(cols, dtype=dtype, seed=4)
+    q, scale = check_fp8(T, x, w, 1e-12, group)
+    assert bool((scale == scale.min()).all()) and float(q.float().abs().max()) >= 16
+
+
 # --------------------------------------------------------------- sampling
 
 
