@@ -4,8 +4,11 @@
 //   s = x + residual,  rstd = 1 / sqrt(mean(s^2) + eps),  y = w s rstd
 //   e4m3 output: scale = max(max|y|, 2^-100) / 448 over a row or a group of
 //   columns, q = y / scale.
-//   gradient:    dx = rstd w dy - s rstd^3 mean(w dy s) + dsum,
-//                dw = sum over rows of dy s rstd
+//   gradient:    dx = rstd (w dy - xhat mean(w dy xhat)) + dsum, xhat = s rstd,
+//                dw = sum over rows of dy xhat
+//
+// No power of rstd is formed: its cube leaves 32 bits where the result does not
+// (rows of rms above 4e12 or below 2e-13).
 //
 // All in 32 bits from the unrounded sum s; each output is rounded once.
 #include <cuda_fp8.h>
@@ -578,7 +581,7 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(const __grid_constant__ 
         }
         row_fold<true, false>(ss, gs, false, red[turn]);  // two buffers: one barrier per row is enough
         const float rstd = rsqrtf(ss * p.per_col + p.eps);
-        const float back = rstd * rstd * rstd * (gs * p.per_col);
+        const float along = rstd * (gs * p.per_col);  // mean(w dy xhat)
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             if (chunks.some(c)) {
@@ -596,9 +599,9 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(const __grid_constant__ 
                 weights.get(c, w);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    const float s = to_f32(ux[h].e[j]), g = to_f32(ug[h].e[j]) * rstd;
-                    dw[c][j] += g * s;
-                    dx[j] += g * w[j] - s * back;
+                    const float xhat = to_f32(ux[h].e[j]) * rstd, g = to_f32(ug[h].e[j]);
+                    dw[c][j] += g * xhat;
+                    dx[j] += rstd * (g * w[j] - xhat * along);
                 }
                 chunks.store(static_cast<T *>(p.dx) + (int64_t)row * p.cols, c, dx);
             }
@@ -646,7 +649,7 @@ template <typename T, int V> __global__ void __launch_bounds__(1024) norm_grad_l
         }
         row_fold<true, false>(ss, gs, false, red[turn]);
         const float rstd = rsqrtf(ss * p.per_col + p.eps);
-        const float back = rstd * rstd * rstd * (gs * p.per_col);
+        const float along = rstd * (gs * p.per_col);  // mean(w dy xhat)
         for (uint32_t col = threadIdx.x * V; col < p.cols; col += blockDim.x * V) {
             float w[V], s[V], g[V], dx[V] = {};
             load_weight<T, V>(p.weight, p.weight_f32, col, w);
@@ -656,8 +659,9 @@ template <typename T, int V> __global__ void __launch_bounds__(1024) norm_grad_l
             float *mine = p.partials ? p.partials + (int64_t)blockIdx.x * p.cols + col : nullptr;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                dx[j] += g[j] * rstd * w[j] - s[j] * back;
-                if (mine) mine[j] = (row == blockIdx.x ? 0.0f : mine[j]) + g[j] * rstd * s[j];
+                const float xhat = s[j] * rstd;
+                dx[j] += rstd * (g[j] * w[j] - xhat * along);
+                if (mine) mine[j] = (row == blockIdx.x ? 0.0f : mine[j]) + g[j] * xhat;
             }
             store_as<T, V>(static_cast<T *>(p.dx) + (int64_t)row * p.cols + col, dx);
         }

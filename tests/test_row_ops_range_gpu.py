@@ -83,6 +83,25 @@ def test_rms_norm_fp8_below_the_least_scale(T, dtype, cols, group):
     assert bool((scale == scale.min()).all()) and float(q.float().abs().max()) >= 16
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols", [(300, 64), (5, 4096), (9, 257), (3, 16384), (2, 33000)])
+def test_rms_norm_backward_of_tiny_and_huge_rows(T, dtype, rows, cols):
+    """Rows whose norm is far from 1: rstd cubed is no number of 32 bits, the gradient is."""
+    dy, w, d = rand(rows, cols, dtype=dtype, seed=1), rand(cols, dtype=dtype, seed=2), rand(rows, cols, dtype=dtype, seed=3)
+    for scale in (1e-17, 1e-13, 1e-12, 1e-6, 1e4, 1e12, 1e13, 1e14, 1e15, 1e16):
+        s = rand(rows, cols, seed=4, scale=scale).to(dtype)
+        for eps in (0.0, 1e-30, 1e-6):
+            for dsum in (None, (d.double() / scale).to(dtype)):
+                ds, dw = T.rms_norm_backward(dy, s, w, eps, dsum=dsum)
+                want, want_w, size, size_w = ref.rms_norm_grads(dy, s, w, eps, dsum)
+                near(ds, want, size, 2 * FOLD)
+                near(dw, want_w, size_w, 2 * FOLD)
+    s[:] = 0  # rows of zeros: dx = w dy / sqrt(eps)
+    ds, dw = T.rms_norm_backward(dy, s, w, 1e-30)
+    near(ds, dy.double() * w.double() * 1e15)
+    assert bool((dw == 0).all())
+
+
 # --------------------------------------------------------------- sampling
 
 
