@@ -291,6 +291,7 @@ route_kernel(const __grid_constant__ RouteParams p) {
         for (int j = 0; j < N; ++j) {
             c[j] = c[j] > -INFINITY ? score(c[j]) + b[j] : -INFINITY;
             key[j] = key_of(c[j], j);
+            if (!key[j]) c[j] = -INFINITY;  // a NaN bias: no minimum or maximum passes over it both ways
         }
     } else {
 #pragma unroll

@@ -102,6 +102,25 @@ def test_rms_norm_backward_of_tiny_and_huge_rows(T, dtype, rows, cols):
     assert bool((dw == 0).all())
 
 
+# ---------------------------------------------------------------- routing
+
+
+@pytest.mark.parametrize("experts,groups,kept,k", [(32, 4, 2, 4), (64, 8, 3, 4), (256, 8, 4, 8), (512, 16, 3, 6), (1024, 8, 2, 8),
+                                                   (60, 5, 2, 4), (300, 4, 2, 8)])
+def test_route_nan_bias_with_groups(T, experts, groups, kept, k):
+    """An expert of NaN bias is not chosen, nor is it worth anything to its group."""
+    logits, bias = rand(150, experts, seed=experts), rand(experts, seed=1, scale=0.2)
+    size = experts // groups
+    bias[1::5] = float("nan")
+    bias[2 * size:3 * size - 1] = float("nan")  # one expert left in this group
+    bias[3 * size:4 * size] = float("nan")      # and none in this
+    bias[size] = float("-inf")
+    for score in ("softmax", "sigmoid"):
+        for top in (1, 2):
+            _, picks = check_route(T, logits, k, score=score, bias=bias, groups=groups, groups_kept=kept, group_top=top)
+            assert not bool(bias[picks[picks >= 0].long()].isnan().any())
+
+
 # --------------------------------------------------------------- sampling
 
 
