@@ -295,7 +295,10 @@ route_kernel(const __grid_constant__ RouteParams p) {
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j) key[j] = key_of(c[j], j);
+        for (int j = 0; j < N; ++j) {
+            key[j] = key_of(c[j], j);
+            if (!key[j]) c[j] = -INFINITY;
+        }
     }
     // Half of what two keys' values may differ by and yet be in the other
     // order: the score's error, a rounding of the sum, a unit of the last kept bit.
@@ -343,9 +346,11 @@ route_kernel(const __grid_constant__ RouteParams p) {
             if (e < p.experts && !(kept >> (e / p.group_size) & 1u)) key[j] = 0;
         }
     }
-    // Best and second of the lane's experts, to value its group by.
+    // Best and second of the lane's experts, to value its group by: of score +
+    // bias, or of the logits, whose order is the scores'.  (Not of the keys,
+    // whose low bits are not the value's.)
     float best = -INFINITY, second = -INFINITY;
-    if (p.group_lanes && p.bias) {
+    if (p.group_lanes && p.groups > 1) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             second = fmaxf(second, fminf(best, c[j]));
@@ -357,10 +362,8 @@ route_kernel(const __grid_constant__ RouteParams p) {
         // A group is a power of two of whole lanes, which share the comparisons.
         float a = best, b = second;
         if (!p.bias) {
-            // Without a bias the order is that of the logits: two scores will do.
-            auto value = [&](uint32_t k) { return k ? score(to_f32(src[lane * N + kLow - (k & kLow)])) : -INFINITY; };
-            a = value(key[0]);
-            b = N > 1 ? value(key[N > 1]) : -INFINITY;
+            a = best > -INFINITY ? score(best) : -INFINITY;
+            b = second > -INFINITY ? score(second) : -INFINITY;
         }
         for (uint32_t d = 1; d < p.group_lanes; d *= 2) {
             const float oa = shfl_xor(a, d), ob = shfl_xor(b, d);

@@ -121,6 +121,37 @@ def test_route_nan_bias_with_groups(T, experts, groups, kept, k):
             assert not bool(bias[picks[picks >= 0].long()].isnan().any())
 
 
+@pytest.mark.parametrize("experts,groups", [(64, 8), (128, 4), (256, 8), (512, 8), (1024, 16), (300, 4), (60, 5)])
+def test_route_groups_of_neighbouring_large_logits(T, experts, groups):
+    """Which group stays hangs on a few units in the last place of logits beside one another."""
+    rows, size = 600, experts // groups
+    per_lane = max(1, 1 << (experts - 1).bit_length() >> 5)  # experts that are held together
+    g = torch.Generator().manual_seed(experts)
+
+    def pick(*high):
+        return [int(torch.randint(0, h, (1,), generator=g)) for h in high]
+
+    logits = torch.zeros(rows, experts)
+    for row in range(rows):
+        base = float(torch.empty(1).uniform_(100, 1000, generator=g))
+        ulp = 2.0 ** (torch.tensor(base).log2().floor().item() - 23)
+        base = float(torch.tensor(base))
+        one, step = pick(groups, groups - 1)
+        other = (one + 1 + step) % groups
+        at = one * size + pick(size)[0] // per_lane * per_lane
+        for j in range(3):  # beside one another in one group
+            logits[row, at + pick(per_lane)[0] if at + per_lane <= (one + 1) * size else at] = base + pick(per_lane + 2)[0] * ulp
+        for j in range(2):  # and anywhere in the other
+            logits[row, other * size + pick(size)[0]] = base + pick(per_lane + 2)[0] * ulp
+    logits[0] = 0.0
+    logits[0, 0], logits[0, 1], logits[0, size] = 1000.0, 1000.0 + 7 * 2.0 ** -14, 1000.0 + 3 * 2.0 ** -14
+    logits = logits.cuda()
+    for score in ("softmax", "sigmoid"):
+        for top in (1, 2):
+            for kept in (1, 2):
+                check_route(T, logits, 2, score=score, groups=groups, groups_kept=kept, group_top=top)
+
+
 # --------------------------------------------------------------- sampling
 
 
