@@ -249,8 +249,10 @@ struct Weigher {
         top = fminf(max, FLT_MAX);
         slope = 16 * 1.4426950408889634 / t;
         slope32 = (float)(2.0 * slope);
-        // Below half a unit; and no -inf, whatever the temperature.
-        floor = fmaxf(__double2float_rd((double)max - (scale_bits + 1.5) * 0.6931471805599453 * t), -FLT_MAX);
+        // Below half a unit; and no -inf, whatever the temperature.  Rounded up:
+        // the next number below may be thousands of T further down, where
+        // mass() has no exponent for it.
+        floor = fmaxf(__double2float_ru((double)max - (scale_bits + 1.5) * 0.6931471805599453 * t), -FLT_MAX);
     }
     // exp((l - max) / T) 2^scale_bits, rounded, for l >= floor (else anything);
     // a unit is at least 2^-45 of the maximum's mass, which is 2^scale_bits.

@@ -275,7 +275,8 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p
     among equals) top_k keeps the first k (0: off), top_p of those the ones before which lies less
     than top_p of their mass (1: off), min_p of those the ones of at least min_p of the largest weight
     (0: off).  The token is the first index whose running sum of kept weights exceeds uniform times
-    their whole; temperature 0 takes the largest.  Each setting is a number or a tensor of one per
+    their whole (a weight below 2^-45 of the largest, 2^-39 in the widest vocabularies, counts as none);
+    temperature 0 takes the largest.  Each setting is a number or a tensor of one per
     row (f32; top_k i32), where values outside its range turn it off (a temperature: take the
     largest).  The answer for a row is the same in any batch.  Returns (tokens i64 [rows], probs f32
     [rows]), the probability among the kept ones; a row of nothing but -inf and NaN has token -1."""

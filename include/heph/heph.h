@@ -565,7 +565,9 @@ heph_status heph_expert_order(int ordinal, const int32_t *picks, uint64_t count,
  * of their mass (1: off), min_p of those the ones with w >= min_p (0: off);
  * the first always stays.  The token is the first index whose running sum of
  * kept w exceeds uniform[row] (in [0, 1)) times the whole; `probs` receives its
- * share of the kept w.  T = 0 takes the first.  Each setting is one value, or
+ * share of the kept w.  Weights are whole numbers of units of 2^-44 of the largest (2^-43 from 2^18
+ * logits on, 2^-42 from 2^19, 2^-38 past 2^20 - 2^16): one below half a unit has no part in any sum
+ * and is not drawn, not even at uniform = 0.  T = 0 takes the first.  Each setting is one value, or
  * a device array with one per row (NULL: the value); in an array a
  * temperature <= 0 or NaN takes the first, and a top_k <= 0, a top_p >= 1 or NaN and
  * a min_p <= 0 or NaN are off.  NaN logits count as -inf; a row of nothing but -inf has token -1

@@ -180,3 +180,44 @@ def test_sample_threshold_among_subnormals_beside_zeros(T):
     # Weights of 1 but for the -9: masses in the same ranges.
     for p in (0.2, 0.5, 0.63, 0.64, 0.9, 0.99):
         check_sample(T, logits, u, top_p=p)
+
+
+def check_sample_to_units(T, logits, u, temperature, top_k=0, top_p=1.0, min_p=0.0):
+    """check_sample for points that a weight below a unit may decide (u = 0 before all).
+
+    Weights are whole numbers of units of 2^-44 of the largest (vocabularies up to 2^17), each rounded by
+    half a unit and made to 1e-14 < 2^-46 of it: a running sum of n weights is within n 2^-44 of the 64-bit
+    one, as is the whole.  A token whose running sums, before it and with it, hold the point to within
+    that is right; where no border is that near there is only one."""
+    tokens, probs = T.sample_tokens(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    for row, (token, prob) in enumerate(zip(tokens.tolist(), probs.tolist())):
+        l = logits[row].double().cpu()
+        w = torch.exp((l - l.max()) / temperature)
+        index = torch.sort(l, descending=True, stable=True).indices[: top_k or len(l)]
+        before = torch.cumsum(w[index], 0) - w[index]
+        stay = (before < top_p * w[index].sum()) & (w[index] >= min_p)
+        stay[0] = True
+        kept = torch.zeros_like(w).index_copy(0, index[stay], w[index[stay]])
+        run, off = torch.cumsum(kept, 0), 2 * len(l) * 2.0 ** -44
+        point = float(u[row]) * float(run[-1])
+        assert float(run[token] - kept[token]) <= point + off and float(run[token]) > point - off
+        assert bool((index[stay] == token).any())
+        want = float(kept[token] / run[-1])
+        assert abs(prob - want) <= want * (2.0 ** -24 + 2.0 ** -30) + len(l) * 2.0 ** -44
+
+
+@pytest.mark.parametrize("vocab", [700, 9001])
+def test_sample_neighbours_of_the_largest_at_small_temperatures(T, vocab):
+    """The number next below the largest logit may be any number of temperatures away: it has no weight
+    where that is far."""
+    u = torch.tensor([0.0, 0.3, 0.6, 0.999], device="cuda")
+    for top in (1.0, 9.0, -3.0, 1e4, 1e10, 1e12, 3e38):
+        logits = (rand(4, vocab, seed=1) - 8) * abs(top)
+        top = torch.tensor(top, device="cuda")
+        logits[:, 5] = torch.nextafter(top, -top.abs() * 2)
+        logits[:, 11:600:7] = logits[:, 5:6]
+        logits[:, [300, 650]] = top
+        step = float(top.double() - logits[0, 5].double())
+        for t in (step / 5e5, step / 59600, step / 3000, step / 1000, step / 100, step / 25, step, 20 * step):
+            for kw in (dict(), dict(top_k=40), dict(top_p=0.8), dict(min_p=0.01)):
+                check_sample_to_units(T, logits, u, t, **kw)
