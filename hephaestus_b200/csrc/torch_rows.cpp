@@ -295,6 +295,12 @@ heph_route_score route_score(PyObject *o) {
     refuse("unknown routing score" + (name ? " '" + std::string(name) + "'" : std::string()));
 }
 
+// Before the numbers become 32-bit ones of the C ABI.
+void check_choice(const char *op, int64_t k, int64_t experts) {
+    if (experts < 1 || experts > 1024 || k < 1 || k > 32 || k > experts)
+        refuse(std::string(op) + " chooses 1 to 32 of up to 1024 experts, not " + std::to_string(k) + " of " + std::to_string(experts));
+}
+
 // route_experts(logits, k, score, bias, groups, groups_kept, group_top, renormalize, scale)
 PyObject *route_experts(PyObject *const *args) {
     const at::Tensor &logits = tensor(args[0], "logits");
@@ -304,8 +310,7 @@ PyObject *route_experts(PyObject *const *args) {
     heph_row_dtype dtype;
     row_dtype(logits.scalar_type(), &dtype);
     const int64_t k = whole(args[1], "k", INT64_MIN, INT64_MAX);
-    if (m.cols < 1 || m.cols > 1024 || k < 1 || k > 32 || k > m.cols)
-        refuse("route_experts chooses 1 to 32 of up to 1024 experts, not " + std::to_string(k) + " of " + std::to_string(m.cols));
+    check_choice("route_experts", k, m.cols);
     const void *b = bias ? vector_of("bias", *bias, m.cols, {at::kFloat}) : nullptr;
     const uint32_t groups = (uint32_t)whole(args[4], "groups", 0, UINT32_MAX), kept = (uint32_t)whole(args[5], "groups_kept", 0, UINT32_MAX);
     const uint32_t top = (uint32_t)whole(args[6], "group_top", 0, UINT32_MAX);
@@ -329,6 +334,7 @@ PyObject *route_experts_backward(PyObject *const *args) {
     heph_row_dtype dtype;
     row_dtype(logits.scalar_type(), &dtype);
     if (experts.dim() != logits.dim()) refuse("experts must have the logits' leading dimensions");
+    check_choice("route_experts_backward", experts.size(-1), m.cols);
     const auto shape = with_columns(logits, experts.size(-1));
     const at::IntArrayRef want(shape);
     const Matrix g = rows_of("dweights", dweights, at::kFloat, &want), p = rows_of("experts", experts, at::kInt, &want);
