@@ -11,6 +11,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -100,6 +101,9 @@ int64_t whole(PyObject *o, const char *name, int64_t low, int64_t high) {
 void check_grad(const char *name, const at::Tensor &t) {
     if (t.requires_grad() && c10::GradMode::is_enabled())
         refuse(std::string(name) + " asks for a gradient, which these calls do not record: detach it, or use torch.no_grad()");
+    // A dual tensor of forward-mode differentiation, which no_grad() does not turn off (level 0 is the only one).
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+        refuse(std::string(name) + " has a tangent, which these calls do not carry: take its primal (torch.autograd.forward_ad.unpack_dual)");
 }
 
 // What the tensor holds is what its memory says.

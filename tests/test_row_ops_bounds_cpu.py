@@ -25,3 +25,25 @@ def test_sizes_past_32_bits():
     refused(f"2 of {past}", T.route_experts, wide(past, torch.bfloat16), 2)
     refused("1 to 1024", T.expert_order, p, past)
     refused("[rows, vocabulary]", T.sample_tokens, wide(past, torch.bfloat16), torch.zeros(1))
+
+
+def test_forward_mode_tensors_are_refused():
+    """A tangent is not dropped in silence."""
+    from torch.autograd import forward_ad
+    x, w = torch.ones(4, 64), torch.ones(64)
+    p = torch.zeros(4, 2, dtype=torch.int32)
+    with forward_ad.dual_level():
+        d, dw = forward_ad.make_dual(x, x), forward_ad.make_dual(w, w)
+        du = forward_ad.make_dual(torch.zeros(4), torch.ones(4))
+        dg = forward_ad.make_dual(x[:, :2].clone(), x[:, :2].clone())
+        for call, args, kw in ((T.rms_norm, (d,), {}), (T.rms_norm, (x, dw), {}), (T.rms_norm, (x,), dict(residual=d)),
+                               (T.rms_norm_fp8, (d,), {}), (T.rms_norm_backward, (d, x), {}), (T.rms_norm_backward, (x, d), {}),
+                               (T.rms_norm_backward, (x, x), dict(dsum=d)), (T.route_experts, (d, 2), {}),
+                               (T.route_experts, (x, 2), dict(bias=dw)), (T.route_experts_backward, (dg, x, p), {}),
+                               (T.route_experts_backward, (x[:, :2], d, p), {}), (T.sample_tokens, (d, torch.zeros(4)), {}),
+                               (T.sample_tokens, (x, du), {}), (T.sample_tokens, (x, torch.zeros(4)), dict(temperature=du))):
+            refused("has a tangent", call, *args, **kw)
+            with torch.no_grad():
+                refused("has a tangent", call, *args, **kw)
+        refused("needs CUDA tensors", T.rms_norm, forward_ad.unpack_dual(d).primal)
+    refused("needs CUDA tensors", T.rms_norm, d)  # outside its level it is the primal
