@@ -67,7 +67,8 @@ def _compile(src: str, verbose_ptxas: bool) -> str:
 def build_torch_module(force: bool = False) -> str | None:
     """``_torch_rows.so``: the torch boundary of the row operators, beside LIB.
 
-    None, and no module, without a CUDA build of torch: LIB does not need one."""
+    None, and no module, without a CUDA build of torch: LIB does not need one.
+    Where it does not compile, none is left of older sources either."""
     src = os.path.join(CSRC, "torch_rows.cpp")
     spec = importlib.util.find_spec("torch")
     torch_dir = os.path.dirname(spec.origin) if spec else ""
@@ -76,10 +77,13 @@ def build_torch_module(force: bool = False) -> str | None:
     newest_dep = max(os.path.getmtime(p) for p in [src, __file__, spec.origin] + headers())
     if os.path.exists(TORCH_MODULE) and os.path.getmtime(TORCH_MODULE) >= newest_dep and not force:
         return TORCH_MODULE
+    import torch
+
     cuda_home = os.path.dirname(os.path.dirname(nvcc()))
     lib_dir = os.path.join(torch_dir, "lib")
     tmp = TORCH_MODULE + ".tmp"
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-fPIC", "-shared", "-Wall", "-D_GLIBCXX_USE_CXX11_ABI=1",
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-fPIC", "-shared", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
            "-I", INCLUDE, "-isystem", os.path.join(torch_dir, "include"),
            "-isystem", os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
            "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(cuda_home, "include"),
@@ -87,9 +91,22 @@ def build_torch_module(force: bool = False) -> str | None:
            "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{lib_dir}"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
+        if os.path.exists(TORCH_MODULE):
+            os.remove(TORCH_MODULE)
         raise RuntimeError(f"{cmd[0]} failed on {src}:\n{res.stderr}")
     os.replace(tmp, TORCH_MODULE)
     return TORCH_MODULE
+
+
+def _torch_module_or_note(force: bool = False) -> None:
+    """build_torch_module, or a line on stderr that says why it is left out: LIB is complete without it."""
+    try:
+        made = build_torch_module(force)
+        why = "no CUDA build of torch is installed"
+    except (RuntimeError, OSError, ImportError) as e:
+        made, why = None, str(e)
+    if made is None:
+        sys.stderr.write(f"{os.path.basename(TORCH_MODULE)} (torch_ops' row operators) is left out: {why}\n")
 
 
 def build(verbose_ptxas: bool = False, force: bool = False) -> str:
@@ -102,7 +119,7 @@ def build(verbose_ptxas: bool = False, force: bool = False) -> str:
         objs = list(ex.map(lambda s: _compile(s, verbose_ptxas), srcs))
     if (os.path.exists(LIB) and not force and
             os.path.getmtime(LIB) >= max(os.path.getmtime(o) for o in objs)):
-        build_torch_module()
+        _torch_module_or_note()
         return LIB
     tmp = LIB + ".tmp"
     cmd = [nvcc(), *ARCH, "-shared", "-o", tmp, *objs, "-ldl"]
@@ -110,7 +127,7 @@ def build(verbose_ptxas: bool = False, force: bool = False) -> str:
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stderr}")
     os.replace(tmp, LIB)
-    build_torch_module(force)
+    _torch_module_or_note(force)
     return LIB
 
 

@@ -20,8 +20,19 @@ import ctypes
 import torch
 
 from . import _native as N
-from . import _torch_rows
 from .core import CudaBuffer, CudaDevice, InvalidConfiguration, Layout, StridedView, check
+
+try:
+    from . import _torch_rows
+except ImportError as e:  # all but the row operators needs the library alone
+
+    class _Absent:
+        why = str(e)
+
+        def __getattr__(self, name):
+            raise ImportError(f"{name} needs hephaestus_b200/_torch_rows.so, which build.py makes for the installed torch: {self.why}")
+
+    _torch_rows = _Absent()
 
 _TORCH_DTYPES = {torch.float32: N.F32, torch.float64: N.F64, torch.int32: N.I32, torch.int64: N.I64}
 if hasattr(torch, "uint32"):
