@@ -1,6 +1,7 @@
 // row_abi.cu — the C ABI of the language-model row operators: every check of
 // their arguments, the device they run on, and the launch.  A refused call
 // touches no device.
+#include <cfloat>
 #include <cmath>
 #include <exception>
 
@@ -104,6 +105,8 @@ heph_status check_norm(const char *op, heph_row_dtype dtype, heph_row_dtype weig
     if (weight && weight_dtype != dtype && weight_dtype != HEPH_ROW_F32)
         return refuse(std::string(op) + " takes a weight of the rows' type or f32");
     if (!(eps >= 0.0) || std::isinf(eps)) return refuse(std::string(op) + " takes a finite eps of 0 or more");
+    // The kernels have it in 32 bits, where a smaller one is 0 (and a row of zeros 0 / 0) and a larger one infinite.
+    if (eps > FLT_MAX || (eps > 0.0 && eps < FLT_MIN)) return refuse(std::string(op) + " takes an eps of 0 or within the normal f32 numbers");
     if (cols == 0) return refuse(std::string(op) + " is undefined for rows of no columns");
     if (rows > kMaxRows || cols > kMaxCols) return refuse(std::string(op) + " rows or columns out of range");
     return check_matrix("weight", weight, weight ? 1 : 0, cols, 0, row_dtype_size(weight_dtype));

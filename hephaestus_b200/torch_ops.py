@@ -225,8 +225,8 @@ def norm_max(t):
 def rms_norm(x, weight=None, eps=1e-6, *, residual=None):
     """[EXT] y = weight * s / sqrt(mean(s^2) + eps) over the last dimension, s = x (+ residual).
 
-    x: f32, bf16 or f16; weight: of x's type or f32 (None: ones).  Returns y, or (y, s) with a
-    residual; both in x's type, each rounded once."""
+    x: f32, bf16 or f16; weight: of x's type or f32 (None: ones); eps: 0 or a normal f32 number.
+    Returns y, or (y, s) with a residual; both in x's type, each rounded once."""
     return _torch_rows.rms_norm(x, weight, eps, residual)
 
 

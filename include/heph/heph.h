@@ -494,6 +494,8 @@ typedef enum heph_row_dtype {
 /* Root-mean-square norm: s = x + residual (NULL: x), y = weight * s /
  * sqrt(mean(s^2) + eps), a row of `sum` receives s.  weight: `cols` elements
  * of the rows' type or f32, NULL for ones.  s is not rounded before the norm.
+ * eps: 0, or within the normal f32 numbers.  The sum of a row's squares is held in f32: where it passes the
+ * largest (an rms of 1.8e19 / sqrt(cols)), y is 0.
  * A row that holds a NaN or an infinity has NaN in y where IEEE has it. */
 heph_status heph_rms_norm(int ordinal, heph_row_dtype dtype, const void *x, int64_t x_stride,
                           const void *residual, int64_t residual_stride, const void *weight,

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from hephaestus_b200 import InvalidConfiguration
+from hephaestus_b200 import _native as N
 from hephaestus_b200 import torch_ops as T
 
 
@@ -47,3 +48,16 @@ def test_forward_mode_tensors_are_refused():
                 refused("has a tangent", call, *args, **kw)
         refused("needs CUDA tensors", T.rms_norm, forward_ad.unpack_dual(d).primal)
     refused("needs CUDA tensors", T.rms_norm, d)  # outside its level it is the primal
+
+
+@pytest.mark.parametrize("eps,good", [(0.0, True), (1.2e-38, True), (3.4e38, True), (1e-39, False), (1e-60, False), (3.5e38, False),
+                                      (1e300, False)])
+def test_an_eps_that_32_bits_do_not_hold(eps, good):
+    """As 32 bits a smaller one is 0, and a row of zeros 0 / 0; a larger one is infinite."""
+    a = 0x1000000  # an address that nothing reads: without rows nothing is done
+    norm = N.lib.heph_rms_norm(0, N.ROW_F32, a, 64, None, 0, None, N.ROW_F32, eps, 0, 64, 2 * a, None, None)
+    fp8 = N.lib.heph_rms_norm_fp8(0, N.ROW_F32, a, 64, None, 0, None, N.ROW_F32, eps, 0, 64, 0, 2 * a, 3 * a, None, None)
+    grad = N.lib.heph_rms_norm_backward(0, N.ROW_F32, a, 64, a, 64, None, 0, None, N.ROW_F32, eps, 0, 64, 2 * a, None, None, 0, None)
+    assert {norm, fp8, grad} == {N.OK if good else N.INVALID_CONFIGURATION}
+    if not good:
+        assert "normal f32 numbers" in N.last_error()
