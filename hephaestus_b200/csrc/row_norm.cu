@@ -321,6 +321,21 @@ norm_kernel(const __grid_constant__ NormParams p) {
     finish_row<T, V, C, S, SHIFTED>(p, row, chunks, v, ss, amax, gmax, group_max);
 }
 
+// A thread's sum over a long row, up to 2^14 terms: in runs of 128, so that no
+// chain of additions is longer (one chain of equal terms is off by 2e-4 there).
+struct LongSum {
+    float sum = 0.0f, run = 0.0f;
+    uint32_t count = 0;
+    __device__ __forceinline__ void add(float v) {
+        run += v;
+        if ((++count & 127u) == 0) {
+            sum += run;
+            run = 0.0f;
+        }
+    }
+    __device__ __forceinline__ float total() const { return sum + run; }
+};
+
 // Rows too long for the registers, or of operands with no common boundaries:
 // read twice, the second time from L2.
 template <typename T, int V, bool FP8> __global__ void __launch_bounds__(1024) norm_long_kernel(const __grid_constant__ NormParams p) {
@@ -344,14 +359,16 @@ template <typename T, int V, bool FP8> __global__ void __launch_bounds__(1024) n
             for (int j = 0; j < V; ++j) v[j] += to_f32(r.e[j]);
         }
     };
-    float ss = 0.0f, amax = 0.0f;
+    LongSum squares;
+    float amax = 0.0f;
 #pragma unroll 2
     for (uint32_t col = t * V; col < p.cols; col += blockDim.x * V) {
-        float v[V], w[V], vmax = 0.0f;
+        float v[V], w[V], vmax = 0.0f, some = 0.0f;
         load(col, v);
         if (res) store_as<T, V>(static_cast<T *>(p.sum) + (int64_t)row * p.cols + col, v);
 #pragma unroll
-        for (int j = 0; j < V; ++j) ss += v[j] * v[j];
+        for (int j = 0; j < V; ++j) some += v[j] * v[j];
+        squares.add(some);
         if constexpr (FP8) {
             load_weight<T, V>(p.weight, p.weight_f32, col, w);
 #pragma unroll
@@ -360,6 +377,7 @@ template <typename T, int V, bool FP8> __global__ void __launch_bounds__(1024) n
             if (by_group) shared_max(&group_max[col >> p.group_shift], vmax);
         }
     }
+    float ss = squares.total();
     row_fold<FP8, true>(ss, amax, false, red);
     if (by_group) __syncthreads();
     const float rstd = rsqrtf(ss * p.per_col + p.eps);
@@ -635,9 +653,9 @@ template <typename T, int V> __global__ void __launch_bounds__(1024) norm_grad_l
         for (int j = 0; j < V; ++j) v[j] = to_f32(u.e[j]);
     };
     for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
-        float ss = 0.0f, gs = 0.0f;
+        LongSum squares, products;
         for (uint32_t col = threadIdx.x * V; col < p.cols; col += blockDim.x * V) {
-            float w[V], s[V], g[V];
+            float w[V], s[V], g[V], ss = 0.0f, gs = 0.0f;
             load_weight<T, V>(p.weight, p.weight_f32, col, w);
             load(p.x, row * p.x_stride + col, s);
             load(p.dy, row * p.dy_stride + col, g);
@@ -646,7 +664,10 @@ template <typename T, int V> __global__ void __launch_bounds__(1024) norm_grad_l
                 ss += s[j] * s[j];
                 gs += g[j] * w[j] * s[j];
             }
+            squares.add(ss);
+            products.add(gs);
         }
+        float ss = squares.total(), gs = products.total();
         row_fold<true, false>(ss, gs, false, red[turn]);
         const float rstd = rsqrtf(ss * p.per_col + p.eps);
         const float along = rstd * (gs * p.per_col);  // mean(w dy xhat)

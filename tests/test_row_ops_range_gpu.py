@@ -102,6 +102,32 @@ def test_rms_norm_backward_of_tiny_and_huge_rows(T, dtype, rows, cols):
     assert bool((dw == 0).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cols", [(1 << 24), (1 << 24) - 1, (1 << 22) + 8])
+def test_rms_norm_of_the_widest_rows(T, dtype, cols):
+    """Sums of up to 2^24 terms, equal ones, whose roundings all go one way.
+
+    A thread adds 2^14 terms at most in chains of 128, 128 and 8, and the block in 10 levels: fewer than 288 roundings, or
+    3 FOLD, of a sum.  y has half of the sum of squares' (a root); dx three halves of it and one of the other sum."""
+    x = torch.full((1, cols), 0.37, device="cuda").to(dtype)
+    dy = torch.full((1, cols), 0.11, device="cuda").to(dtype)
+    for apart in (False, True):
+        if apart:  # rows off every vector boundary of one another
+            memory = torch.empty(cols + 8, device="cuda", dtype=dtype)
+            memory[1:cols + 1] = x[0]
+            x = memory[1:cols + 1].unsqueeze(0)
+        want, s = ref.rms_norm(x, None, 1e-6, dy)
+        y, total = T.rms_norm(x, None, residual=dy)
+        near(y, want, chain=3 * FOLD)
+        q, scale = T.rms_norm_fp8(x, None, residual=dy)[:2]
+        near(scale, ref.scales(want, None), chain=3 * FOLD)
+        assert bool((q.float() == 448).all())  # all equal to the largest
+        del q, total, want, s
+        dx = T.rms_norm_backward(dy, x, None, 1e-6)[0]
+        want, _, size, _ = ref.rms_norm_grads(dy, x, None, 1e-6)
+        near(dx, want, size, 8 * FOLD)
+
+
 # ---------------------------------------------------------------- routing
 
 
