@@ -472,6 +472,8 @@ struct NormGradParams {
 // when it is read would hold up the block at every row) and masked when read.
 template <int C> constexpr int kRowStages = C >= 4 ? 2 : 4;
 
+constexpr uint32_t kDweightRun = 256;  // rows whose terms of dw are added in one chain
+
 template <typename T, int V, int C, int OPERANDS, bool SHIFTED> struct RowRing {
     static constexpr int kStages = kRowStages<C>;
     const T *base[OPERANDS];  // null: absent
@@ -557,7 +559,8 @@ template <typename T, int V, int C, bool SHIFTED> struct RowWeights {
 // Block b takes rows b, b + gridDim.x, ... (SHIFTED: gridDim.x is a multiple of V
 // or covers the rows, so that all of a block's rows start the same distance
 // past a boundary); its share of dw stays in registers (each thread keeps its
-// columns) and goes out once.
+// columns) and goes out at the end, and before that after every kDweightRun
+// rows: one chain over 2^20 rows and more is off by 1e-5 of terms that are alike.
 //
 // Measured at 8192 x 4096 bf16 with dsum: 104 us with rows loaded when they
 // are worked on, 51 us through the ring (5.3 TB/s) and 5 for the sum of the
@@ -571,88 +574,103 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(const __grid_constant__ 
     const Chunks<V, C, SHIFTED> chunks(p.cols, static_cast<const T *>(p.x) + blockIdx.x * p.x_stride, sizeof(T));
     const RowWeights<T, V, C, SHIFTED> weights(p.weight, p.weight_f32, chunks);
     RowRing<T, V, C, 3, SHIFTED> ring({p.x, p.dy, p.dsum}, {p.x_stride, p.dy_stride, p.dsum_stride}, p.rows, chunks, staged);
-    float dw[C][V];
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int j = 0; j < V; ++j) dw[c][j] = 0.0f;
     uint32_t turn = 0;
-    for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
-        ring.next(row);
-        float ss = 0.0f, gs = 0.0f;
-        Pack<T, V> ux[kHeld ? C : 1], ug[kHeld ? C : 1];
+    for (uint32_t row = blockIdx.x; row < p.rows;) {
+        const bool first = row == blockIdx.x;
+        const uint32_t stop = min(p.rows, row + kDweightRun * gridDim.x);
+        float dw[C][V];
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            if (chunks.some(c)) {
-                const int h = kHeld ? c : 0;
-                ux[h] = ring.get(0, c);
-                ug[h] = ring.get(1, c);
-                float w[V];
-                weights.get(c, w);
+        for (int c = 0; c < C; ++c)
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float s = to_f32(ux[h].e[j]);
-                    ss += s * s;
-                    gs += to_f32(ug[h].e[j]) * w[j] * s;
+            for (int j = 0; j < V; ++j) dw[c][j] = 0.0f;
+        for (; row < stop; row += gridDim.x, turn ^= 1) {
+            ring.next(row);
+            float ss = 0.0f, gs = 0.0f;
+            Pack<T, V> ux[kHeld ? C : 1], ug[kHeld ? C : 1];
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                if (chunks.some(c)) {
+                    const int h = kHeld ? c : 0;
+                    ux[h] = ring.get(0, c);
+                    ug[h] = ring.get(1, c);
+                    float w[V];
+                    weights.get(c, w);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        const float s = to_f32(ux[h].e[j]);
+                        ss += s * s;
+                        gs += to_f32(ug[h].e[j]) * w[j] * s;
+                    }
                 }
             }
+            row_fold<true, false>(ss, gs, false, red[turn]);  // two buffers: one barrier per row is enough
+            const float rstd = rsqrtf(ss * p.per_col + p.eps);
+            const float along = rstd * (gs * p.per_col);  // mean(w dy xhat)
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                if (chunks.some(c)) {
+                    const int h = kHeld ? c : 0;
+                    if (!kHeld) {
+                        ux[0] = ring.get(0, c);
+                        ug[0] = ring.get(1, c);
+                    }
+                    float w[V], dx[V] = {};
+                    if (p.dsum) {
+                        const Pack<T, V> u = ring.get(2, c);
+#pragma unroll
+                        for (int j = 0; j < V; ++j) dx[j] = to_f32(u.e[j]);
+                    }
+                    weights.get(c, w);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        const float xhat = to_f32(ux[h].e[j]) * rstd, g = to_f32(ug[h].e[j]);
+                        dw[c][j] += g * xhat;
+                        dx[j] += rstd * (g * w[j] - xhat * along);
+                    }
+                    chunks.store(static_cast<T *>(p.dx) + (int64_t)row * p.cols, c, dx);
+                }
+            }
+            ring.done();
         }
-        row_fold<true, false>(ss, gs, false, red[turn]);  // two buffers: one barrier per row is enough
-        const float rstd = rsqrtf(ss * p.per_col + p.eps);
-        const float along = rstd * (gs * p.per_col);  // mean(w dy xhat)
+        if (!p.partials) continue;
+        float *mine = p.partials + (int64_t)blockIdx.x * p.cols;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            if (chunks.some(c)) {
-                const int h = kHeld ? c : 0;
-                if (!kHeld) {
-                    ux[0] = ring.get(0, c);
-                    ug[0] = ring.get(1, c);
-                }
-                float w[V], dx[V] = {};
-                if (p.dsum) {
-                    const Pack<T, V> u = ring.get(2, c);
+            const uint32_t col = chunks.first(c);
+            if (!chunks.some(c)) continue;
+            if (!first) {
 #pragma unroll
-                    for (int j = 0; j < V; ++j) dx[j] = to_f32(u.e[j]);
-                }
-                weights.get(c, w);
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float xhat = to_f32(ux[h].e[j]) * rstd, g = to_f32(ug[h].e[j]);
-                    dw[c][j] += g * xhat;
-                    dx[j] += rstd * (g * w[j] - xhat * along);
-                }
-                chunks.store(static_cast<T *>(p.dx) + (int64_t)row * p.cols, c, dx);
+                for (int j = 0; j < V; ++j)
+                    if (chunks.has(col, j)) dw[c][j] += mine[col + j];
             }
-        }
-        ring.done();
-    }
-    if (!p.partials) return;
-    float *mine = p.partials + (int64_t)blockIdx.x * p.cols;
+            if constexpr (!SHIFTED) {
+                store_as<float, V>(mine + col, dw[c]);
+            } else {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const uint32_t col = chunks.first(c);
-        if (!chunks.some(c)) continue;
-        if constexpr (!SHIFTED) {
-            store_as<float, V>(mine + col, dw[c]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (chunks.has(col, j)) mine[col + j] = dw[c][j];
+                for (int j = 0; j < V; ++j)
+                    if (chunks.has(col, j)) mine[col + j] = dw[c][j];
+            }
         }
     }
 }
 
 // Rows too long for the registers: read twice; the block's share of dw is
-// gathered in its own row of `partials`, each thread its own columns.
+// gathered in its own row of `partials`, each thread its own columns.  Blocks
+// of more than kDweightRun rows gather those in a second row first (there are
+// two for each block then: launch_rms_norm_backward).
 template <typename T, int V> __global__ void __launch_bounds__(1024) norm_grad_long_kernel(const __grid_constant__ NormGradParams p) {
     __shared__ float2 red[2][32];
-    uint32_t turn = 0;
+    const bool runs = p.rows > kDweightRun * (uint64_t)gridDim.x;
+    float *const whole = p.partials + (int64_t)blockIdx.x * p.cols;
+    float *const gather = whole + (runs ? (int64_t)gridDim.x * p.cols : 0);
+    uint32_t turn = 0, done = 0;  // rows of this block that are done
     auto load = [](const void *src, int64_t at, float (&v)[V]) {
         const auto u = *reinterpret_cast<const Pack<T, V> *>(static_cast<const T *>(src) + at);
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] = to_f32(u.e[j]);
     };
-    for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+    for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1, ++done) {
+        const bool fresh = done % kDweightRun == 0, give = runs && (done % kDweightRun == kDweightRun - 1 || row + gridDim.x >= p.rows);
         LongSum squares, products;
         for (uint32_t col = threadIdx.x * V; col < p.cols; col += blockDim.x * V) {
             float w[V], s[V], g[V], ss = 0.0f, gs = 0.0f;
@@ -677,12 +695,14 @@ template <typename T, int V> __global__ void __launch_bounds__(1024) norm_grad_l
             load(p.x, row * p.x_stride + col, s);
             load(p.dy, row * p.dy_stride + col, g);
             if (p.dsum) load(p.dsum, row * p.dsum_stride + col, dx);
-            float *mine = p.partials ? p.partials + (int64_t)blockIdx.x * p.cols + col : nullptr;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const float xhat = s[j] * rstd;
                 dx[j] += rstd * (g[j] * w[j] - xhat * along);
-                if (mine) mine[j] = (row == blockIdx.x ? 0.0f : mine[j]) + g[j] * xhat;
+                if (!p.partials) continue;
+                const float run = (fresh ? 0.0f : gather[col + j]) + g[j] * xhat;
+                if (give) whole[col + j] = (done < kDweightRun ? 0.0f : whole[col + j]) + run;
+                else gather[col + j] = run;
             }
             store_as<T, V>(static_cast<T *>(p.dx) + (int64_t)row * p.cols + col, dx);
         }
@@ -772,7 +792,8 @@ heph_status launch_rms_norm(const NormArgs &a, cudaStream_t stream) {
 }
 
 // The most blocks that launch_norm_grad starts (4 an SM for rows of up to 192
-// threads, else 3), in whole vectors' worth.
+// threads, else 3), in whole vectors' worth.  norm_grad_long_kernel, of one
+// block an SM, has two rows of partials for each where the blocks have more rows than one.
 uint32_t norm_grad_partials(uint32_t rows, uint32_t cols, int sm_count) {
     const uint32_t most = (cols <= 3000 ? 4 : 3) * (uint32_t)sm_count;
     return rows < most ? rows : most / 8 * 8;

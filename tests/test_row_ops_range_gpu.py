@@ -128,6 +128,26 @@ def test_rms_norm_of_the_widest_rows(T, dtype, cols):
         near(dx, want, size, 8 * FOLD)
 
 
+@pytest.mark.parametrize("rows,cols", [((1 << 24) + 5, 8), ((1 << 24) + 5, 7), (1 << 21, 128), (1 << 21, 127), (300000, 4096)])
+def test_rms_norm_backward_of_many_rows(T, rows, cols):
+    """The weight's gradient is a sum over the rows: of like terms, whose roundings all go one way.
+
+    A block has at most 2^24 / 148 rows, added in chains of 256, these in one of 443, and the blocks' shares in chains
+    of 19 and a tree: fewer than 800 roundings, beside those of a term: 9 FOLD."""
+    x = torch.full((1, cols), 0.37, device="cuda")
+    x[:, ::3] = 0.6
+    dy, w = torch.full((1, cols), 0.11, device="cuda"), rand(cols, seed=1)
+    memory = torch.empty(cols + 8, device="cuda")
+    apart = memory[3:cols + 3].copy_(dy[0]).unsqueeze(0)  # off x's vector boundaries
+    ds, want_w, size, size_w = ref.rms_norm_grads(dy, x, w, 1e-6)
+    for g in (dy, apart):
+        got, dw = T.rms_norm_backward(g.expand(rows, cols), x.expand(rows, cols), w, 1e-6)
+        near(dw, want_w * rows, size_w * rows, 9 * FOLD)
+        for i in (0, rows // 2, rows - 1):
+            near(got[i:i + 1], ds, size, 2 * FOLD)
+        del got
+
+
 # ---------------------------------------------------------------- routing
 
 
