@@ -249,8 +249,15 @@ __device__ __forceinline__ void finish_row(const NormParams &p, uint32_t row, co
 // stay in registers between the one read and the one write.  Bound by HBM,
 // and by the bytes in flight that fill it: rows wait for their sums, others
 // load meanwhile, so blocks an SM count.  16384 x 4096 bf16 with residual and
-// e4m3 scales by 128: four blocks (51 registers) 90 us, five 82.5 us (5.7
+// e4m3 scales by 128: four blocks (51 registers) 90 us, five 82.5-84.5 us (5.6
 // TB/s), six spill, 88 us; 5003 x 2049 f16 six blocks 16.4 us, five 17.4.
+// The rule was chosen on these two forms.  Forms with a residual have less
+// room: SHIFTED in the rows' type at six blocks and two chunks of a 16-bit type
+// or four of f32 (40 registers) spill 116-128 bytes a thread, f32 of aligned
+// rows at five (47-48 registers) 16-32.  There fewer blocks are better: 8192 x
+// 3001 with residual, six / five / four blocks, f32 79 / 68 / 64 us, bf16 59.6 /
+// 57.6 / 61.5; 16384 x 4096 f32 with residual, five / four, 164 / 161 us, to
+// e4m3 by 128 148 / 131.
 template <typename T, int V, int C, Scales S, bool RES, bool SHIFTED>
 __global__ void __launch_bounds__(C * V >= 32 ? 512 : 256, C * V >= 32 ? 1 : SHIFTED && S == kNoScales ? 6 : 5)
 norm_kernel(const __grid_constant__ NormParams p) {
@@ -563,8 +570,9 @@ template <typename T, int V, int C, bool SHIFTED> struct RowWeights {
 // rows: one chain over 2^20 rows and more is off by 1e-5 of terms that are alike.
 //
 // Measured at 8192 x 4096 bf16 with dsum: 104 us with rows loaded when they
-// are worked on, 51 us through the ring (5.3 TB/s) and 5 for the sum of the
-// blocks' dw; 8192 x 4095 105 us without dsum.  (The forward norm gains
+// are worked on, 51-53 us through the ring (5.1-5.3 TB/s) and 5 for the sum of the
+// blocks' dw; SHIFTED, without dsum: 8192 x 4095 105 us, x 8191 206; x 12000
+// 154; 2^20 x 128 836 us, a row's barrier and folds for each.  (The forward norm gains
 // nothing by a ring: 16384 x 4096 88 us against 90 without, narrow rows lose.)
 template <typename T, int V, int C, bool SHIFTED>
 __global__ void __launch_bounds__(512) norm_grad_kernel(const __grid_constant__ NormGradParams p) {

@@ -288,7 +288,8 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p
     (0: off).  The token is the first index whose running sum of kept weights exceeds uniform times
     their whole (a weight below 2^-45 of the largest, 2^-39 in the widest vocabularies, counts as none);
     temperature 0 takes the largest.  Each setting is a number or a tensor of one per
-    row (f32; top_k i32), where values outside its range turn it off (a temperature: take the
-    largest).  The answer for a row is the same in any batch.  Returns (tokens i64 [rows], probs f32
+    row (f32; top_k i32), where a top_k <= 0, a top_p >= 1, a min_p <= 0 and NaN are off, a top_p <= 0
+    leaves the first, a min_p >= 1 those equal to the largest, and a temperature <= 0 or NaN takes the
+    largest.  The answer for a row is the same in any batch.  Returns (tokens i64 [rows], probs f32
     [rows]), the probability among the kept ones; a row of nothing but -inf and NaN has token -1."""
     return _torch_rows.sample_tokens(logits, uniform, temperature, top_k, top_p, min_p)

@@ -572,7 +572,8 @@ heph_status heph_expert_order(int ordinal, const int32_t *picks, uint64_t count,
  * and is not drawn, not even at uniform = 0.  T = 0 takes the first.  Each setting is one value, or
  * a device array with one per row (NULL: the value); in an array a
  * temperature <= 0 or NaN takes the first, and a top_k <= 0, a top_p >= 1 or NaN and
- * a min_p <= 0 or NaN are off.  NaN logits count as -inf; a row of nothing but -inf has token -1
+ * a min_p <= 0 or NaN are off (a top_p <= 0 leaves the first, a min_p >= 1 those equal to the largest, an
+ * infinite temperature weighs all alike).  NaN logits count as -inf; a row of nothing but -inf has token -1
  * and prob 0. */
 heph_status heph_sample_tokens(int ordinal, heph_row_dtype dtype, const void *logits, int64_t stride,
                                uint64_t rows, uint32_t vocab, const float *uniform,

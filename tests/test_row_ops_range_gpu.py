@@ -267,3 +267,21 @@ def test_sample_neighbours_of_the_largest_at_small_temperatures(T, vocab):
         for t in (step / 5e5, step / 59600, step / 3000, step / 1000, step / 100, step / 25, step, 20 * step):
             for kw in (dict(), dict(top_k=40), dict(top_p=0.8), dict(min_p=0.01)):
                 check_sample_to_units(T, logits, u, t, **kw)
+
+
+def test_sample_settings_past_their_ends(T):
+    """In arrays, as documented: negative, past one, infinite."""
+    n, v = 8, 5003
+    logits, u = rand(n, v, seed=5, scale=2).round(), torch.rand(n, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+
+    def each(*values):
+        return torch.tensor(values, device="cuda", dtype=torch.float32).repeat(n)[:n]
+    tokens = check_sample(T, logits, u, top_p=each(-0.5, 0.0, -float("inf")))
+    first = torch.sort(logits, dim=1, descending=True, stable=True).indices[:, 0]
+    assert torch.equal(tokens, first)
+    tokens = check_sample(T, logits, u, min_p=each(1.0, 2.0, float("inf")))
+    assert torch.equal(logits.gather(1, tokens.unsqueeze(1))[:, 0], logits.max(1).values)
+    check_sample(T, logits, u, top_p=each(1.5, float("inf")), min_p=each(-1.0, -float("inf")))
+    hot = each(float("inf"))
+    for kw in (dict(), dict(top_k=100), dict(top_p=0.3), dict(top_k=3000, top_p=0.9)):
+        check_sample(T, logits, u, temperature=hot, **kw)
