@@ -250,9 +250,10 @@ template <int N> __device__ __forceinline__ void sort_falling(uint32_t (&v)[N]) 
 }
 
 // Bound by instruction issue: 32768 x 256 f32, sigmoid, bias, 8 groups, takes
-// 36-39 us with 79 % of the issue slots filled and the ALU pipe 71 % busy, 900 warp
-// instructions a row, of which the sort is 38 minima and maxima; without groups
-// 26 (softmax) and 30 us (sigmoid, bias), 32768 x 64 19 us.
+// 35-43 us (by how many rows 64 bits decide) with 79 % of the issue slots filled
+// and the ALU pipe 71 % busy, 900 warp instructions a row, of which the sort is 38
+// minima and maxima; without groups 26 (softmax) and 30 us (sigmoid, bias), 32768 x
+// 64 19 us.
 //
 // A warp per row, lane i holds experts i N ... i N + N - 1.  The choice is
 // made in 32 bits and checked: where a gap that decides something is not
